@@ -29,6 +29,9 @@ HOST_LIB = os.path.join(LIB_DIR, "libspmm_host.so")
 BIN_DIR = os.path.join(PKG_DIR, "bin")
 A4_BIN = os.path.join(BIN_DIR, "a4")
 ARCH = "gfx950"
+# no packed fp32 arithmetic (v_pk_add/mul/fma_f32): some forms of it have given wrong results on
+# these machines now and then, and -O3 makes them from ordinary float code by itself
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc() -> str:
@@ -70,7 +73,7 @@ def build_hip(force: bool = False, verbose: bool = False, out: str = HIP_LIB, ex
         obj_dir = os.path.join(LIB_DIR, "obj" + tag)
         os.makedirs(obj_dir, exist_ok=True)
         flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
-                 "-munsafe-fp-atomics", *extra]
+                 "-munsafe-fp-atomics", *NO_PACKED_FP32, *extra]
         flag_file = os.path.join(obj_dir, "flags")
         same_flags = os.path.exists(flag_file) and open(flag_file).read() == " ".join(flags)
 
@@ -132,7 +135,7 @@ def build_a4(force: bool = False, verbose: bool = False):
         tmp = A4_BIN + ".tmp"
         # system libstdc++ before conda's (older) in the run path
         rpath = ":".join(["$ORIGIN/../lib", "/usr/lib/x86_64-linux-gnu", "/opt/rocm/lib", os.path.join(mpi, "lib")])
-        cmd = [_hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-I", rt, "-I", os.path.join(mpi, "include"),
+        cmd = [_hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", *NO_PACKED_FP32, "-I", rt, "-I", os.path.join(mpi, "include"),
                "-o", tmp] + srcs + [
                "-L", LIB_DIR, "-lspmm_host", "-lspmm_hip", "-L/opt/rocm/lib", "-lrccl", "-lrocprofiler-sdk-roctx",
                # libmpi by path: a -L into conda would also pick conda's old libstdc++ at link time
