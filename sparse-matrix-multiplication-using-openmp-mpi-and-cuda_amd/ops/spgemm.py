@@ -1072,14 +1072,12 @@ _SIDE = {}
 def _side_stream(dev: torch.device) -> "torch.cuda.Stream":
     """One side stream per (device, thread): loopback ranks are threads that
     share a device, and must not interleave their pipelines on one stream.
-    High priority: HIP maps streams onto its GPU_MAX_HW_QUEUES hardware queues
-    round-robin, and a side stream that lands on the main stream's queue runs
-    strictly after it (an R-MAT kernel trace showed every kernel of both on one
-    queue); a different priority is a different queue."""
+    At the default priority like every stream here: work on streams of
+    different priorities has hung these machines."""
     key = (dev.index, threading.get_ident())
     s = _SIDE.get(key)
     if s is None:
-        s = _SIDE[key] = torch.cuda.Stream(dev, priority=-1)
+        s = _SIDE[key] = torch.cuda.Stream(dev)
     return s
 
 
