@@ -1,0 +1,202 @@
+// CPU engine of the operators on rows over a vocabulary (embedding lookup and
+// gradient, token log-probabilities, distillation): the definitions that the
+// gfx950 kernels of embedding.hip and vocab_logits.hip follow, in double inside
+// and fp32 at the borders, OpenMP over rows.
+#include <omp.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <limits>
+#include <numeric>
+#include <vector>
+
+#define SPMM_HOST_EXPORT extern "C" __attribute__((visibility("default")))
+
+namespace {
+
+constexpr double kNoMass = -std::numeric_limits<double>::infinity();
+const float kNan = std::numeric_limits<float>::quiet_NaN();
+
+inline int threads_or_default(int n) { return n > 0 ? n : omp_get_max_threads(); }
+
+// maximum of the numbers (a NaN is passed over; it reaches the sum), and the sum of exp((z - m) / T)
+struct RowSum {
+  double m, z, u;
+};
+inline double origin(double m) { return m == kNoMass ? 0.0 : m; }
+inline RowSum row_sum(const float* z, int64_t V, double inv_t) {
+  double m = kNoMass;
+  for (int64_t j = 0; j < V; ++j)
+    if (z[j] > m) m = z[j];
+  const double o = origin(m);
+  double s = 0, u = 0;
+  for (int64_t j = 0; j < V; ++j) {
+    const double t = (z[j] - o) * inv_t, e = std::exp(t);
+    s += e;
+    if (e != 0) u += e * t;
+  }
+  return RowSum{m, s, u};
+}
+
+// larger logits first (NaN above all), then lower columns
+inline bool before(const float* z, int32_t a, int32_t b) {
+  const bool na = std::isnan(z[a]), nb = std::isnan(z[b]);
+  if (na != nb) return na;
+  if (!na && z[a] != z[b]) return z[a] > z[b];
+  return a < b;
+}
+
+}  // namespace
+
+SPMM_HOST_EXPORT int spmm_cpu_embedding(int64_t n, int64_t V, int64_t D, const float* W, const int64_t* tok,
+                                        double scale, float* Y, int nthreads) {
+#pragma omp parallel for num_threads(threads_or_default(nthreads))
+  for (int64_t i = 0; i < n; ++i) {
+    const int64_t t = tok[i];
+    float* y = Y + i * D;
+    if (t >= 0 && t < V) {
+      for (int64_t d = 0; d < D; ++d) y[d] = (float)(W[t * D + d] * scale);
+    } else {
+      std::fill(y, y + D, t == -1 ? 0.f : kNan);
+    }
+  }
+  return 0;
+}
+
+// dW (fp32, given) += scale * S^T dY
+SPMM_HOST_EXPORT int spmm_cpu_embedding_grad(int64_t n, int64_t V, int64_t D, const float* dY, const int64_t* tok,
+                                             double scale, float* dW, int nthreads) {
+  std::vector<int64_t> pos;
+  pos.reserve((size_t)n);
+  for (int64_t i = 0; i < n; ++i)
+    if (tok[i] >= 0 && tok[i] < V) pos.push_back(i);
+  std::stable_sort(pos.begin(), pos.end(), [&](int64_t a, int64_t b) { return tok[a] < tok[b]; });
+  std::vector<int64_t> start;   // first of each run of equal tokens
+  for (size_t i = 0; i < pos.size(); ++i)
+    if (i == 0 || tok[pos[i]] != tok[pos[i - 1]]) start.push_back((int64_t)i);
+  start.push_back((int64_t)pos.size());
+#pragma omp parallel num_threads(threads_or_default(nthreads))
+  {
+    std::vector<double> acc((size_t)D);
+#pragma omp for schedule(dynamic, 16)
+    for (int64_t r = 0; r < (int64_t)start.size() - 1; ++r) {
+      std::fill(acc.begin(), acc.end(), 0.0);
+      for (int64_t i = start[(size_t)r]; i < start[(size_t)r + 1]; ++i) {
+        const float* x = dY + pos[(size_t)i] * D;
+        for (int64_t d = 0; d < D; ++d) acc[(size_t)d] += x[d];
+      }
+      float* w = dW + tok[pos[(size_t)start[(size_t)r]]] * D;
+      for (int64_t d = 0; d < D; ++d) w[d] = (float)(w[d] + acc[(size_t)d] * scale);
+    }
+  }
+  return 0;
+}
+
+// stat: [n][2] maximum, Z.  top_col / top_val: [n][k].
+SPMM_HOST_EXPORT int spmm_cpu_token_logprobs(int64_t n, int64_t V, const float* z, const int64_t* tok, double inv_t,
+                                             int k, float* logprob, float* entropy, float* stat, int32_t* top_col,
+                                             float* top_val, int nthreads) {
+#pragma omp parallel num_threads(threads_or_default(nthreads))
+  {
+    std::vector<int32_t> idx((size_t)(k > 0 ? V : 0));
+#pragma omp for
+    for (int64_t i = 0; i < n; ++i) {
+      const float* zi = z + i * V;
+      const RowSum r = row_sum(zi, V, inv_t);
+      const double o = origin(r.m), logz = r.z == 0 ? 0.0 : std::log(r.z);
+      const int64_t t = tok[i];
+      logprob[i] = t >= 0 && t < V ? (float)((zi[t] - o) * inv_t - logz) : (t == -1 ? 0.f : kNan);
+      entropy[i] = r.z == 0 ? 0.f : (float)(logz - r.u / r.z);
+      stat[2 * i] = (float)r.m;
+      stat[2 * i + 1] = (float)r.z;
+      if (k > 0) {
+        std::iota(idx.begin(), idx.end(), 0);
+        std::partial_sort(idx.begin(), idx.begin() + k, idx.end(),
+                          [&](int32_t a, int32_t b) { return before(zi, a, b); });
+        for (int j = 0; j < k; ++j) {
+          top_col[i * k + j] = idx[(size_t)j];
+          top_val[i * k + j] = (float)((zi[idx[(size_t)j]] - o) * inv_t - logz);
+        }
+      }
+    }
+  }
+  return 0;
+}
+
+SPMM_HOST_EXPORT int spmm_cpu_token_logprobs_grad(int64_t n, int64_t V, const float* z, const int64_t* tok, double inv_t,
+                                                  const float* entropy, const float* g, const float* h, float* out,
+                                                  int nthreads) {
+#pragma omp parallel for num_threads(threads_or_default(nthreads))
+  for (int64_t i = 0; i < n; ++i) {
+    const float* zi = z + i * V;
+    float* oi = out + i * V;
+    const int64_t t = tok[i];
+    double gi = g && t != -1 ? g[i] * inv_t : 0.0;
+    const double hi = h ? h[i] * inv_t : 0.0;
+    if (gi == 0 && hi == 0) {
+      std::fill(oi, oi + V, 0.f);
+      continue;
+    }
+    if (t < -1 || t >= V) gi = kNan;
+    const RowSum r = row_sum(zi, V, inv_t);
+    const double o = origin(r.m), logz = r.z == 0 ? 0.0 : std::log(r.z);
+    for (int64_t j = 0; j < V; ++j) {
+      const double lq = (zi[j] - o) * inv_t - logz, q = std::exp(lq);
+      oi[j] = (float)((j == t ? gi : 0.0) - gi * q - (q == 0 ? 0.0 : hi * q * (lq + entropy[i])));
+    }
+  }
+  return 0;
+}
+
+// Teacher entries with column -1 are absent; one outside the vocabulary makes
+// the row's loss and gradient NaN.  out (null: loss only) may be z itself.
+SPMM_HOST_EXPORT int spmm_cpu_distill(int64_t n, int64_t V, const float* z, const int64_t* rowptr, const int32_t* col,
+                                      const float* val, int64_t nnz, double inv_t, float* loss, float* stat,
+                                      const float* weight, float* out, int nthreads) {
+#pragma omp parallel num_threads(threads_or_default(nthreads))
+  {
+    std::vector<double> p((size_t)(out ? V : 0));
+#pragma omp for
+    for (int64_t i = 0; i < n; ++i) {
+      const float* zi = z + i * V;
+      const int64_t b = std::min(std::max<int64_t>(rowptr[i], 0), nnz);
+      const int64_t e = std::min(std::max(rowptr[i + 1], b), nnz);
+      double tm = kNoMass, ts = 0;
+      bool bad = false;
+      for (int64_t k = b; k < e; ++k) {
+        bad |= col[k] < -1 || col[k] >= V;
+        if (col[k] != -1 && val[k] > tm) tm = val[k];
+      }
+      const double to = origin(tm);
+      for (int64_t k = b; k < e; ++k)
+        if (col[k] != -1) ts += std::exp((val[k] - to) * inv_t);
+      const RowSum r = row_sum(zi, V, inv_t);
+      const double o = origin(r.m), logz = r.z == 0 ? 0.0 : std::log(r.z);
+      double l = 0;
+      if (out) std::fill(p.begin(), p.end(), 0.0);
+      if (ts != 0 && !bad)
+        for (int64_t k = b; k < e; ++k) {
+          if (col[k] == -1) continue;
+          const double u = (val[k] - to) * inv_t, pk = std::exp(u) / ts;
+          if (pk != 0) l += pk * ((u - std::log(ts)) - ((zi[col[k]] - o) * inv_t - logz));
+          if (out) p[(size_t)col[k]] += pk;
+        }
+      loss[i] = bad ? kNan : (float)l;
+      stat[4 * i] = (float)r.m;
+      stat[4 * i + 1] = bad ? kNan : (float)r.z;
+      stat[4 * i + 2] = (float)to;
+      stat[4 * i + 3] = bad ? kNan : (float)ts;
+      if (!out) continue;
+      const double w = (weight ? weight[i] : 1.0) * inv_t;
+      float* oi = out + i * V;
+      if (w == 0 || (ts == 0 && !bad)) {
+        std::fill(oi, oi + V, 0.f);
+        continue;
+      }
+      for (int64_t j = 0; j < V; ++j)
+        oi[j] = bad ? kNan : (float)(w * ((r.z == 0 ? 0.0 : std::exp((zi[j] - o) * inv_t) / r.z) - p[(size_t)j]));
+    }
+  }
+  return 0;
+}

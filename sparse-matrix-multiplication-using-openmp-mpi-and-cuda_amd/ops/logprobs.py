@@ -1,0 +1,156 @@
+"""Log-probabilities of given tokens, with entropy and the top alternatives.
+
+For each row z of logits over a vocabulary and a temperature T, with
+``q = softmax(z / T)``: ``ln q[token]``, the entropy ``-sum q ln q``, and the k
+largest logits with their log-probabilities as a CSR matrix (n x V, k entries a
+row), which :func:`ops.distill.distill_loss` takes as a teacher.
+
+* Masked logits (-inf) have q = 0 and add nothing to the entropy.  A row of
+  nothing else has q = 0 everywhere, entropy 0 and log-probabilities of -inf.
+* The largest logits come first, the lower column first among equal ones (+0
+  and -0 are equal, NaN is above all numbers); -inf ones are listed too.
+* Token -1 is padding: its log-probability is 0 and has no gradient.  A token
+  outside the vocabulary has NaN, and so has its row's gradient.
+* A NaN or +inf logit makes its row's results NaN.
+* Sums are held in fp32; results are the same in every run.
+
+gfx950 kernels: ``csrc/kernels/vocab_logits.hip``; CPU tensors use the OpenMP
+kernels of ``csrc/host/vocab_cpu.cpp``.  Nothing here waits for the GPU, so
+both directions can be captured into a HIP graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from .. import _native
+from .._native import c_vp
+from . import rows as R
+from .csr import CSR
+
+_native.register_hip("spmm_vocab_ws", C.c_int64, C.c_int64, C.c_int, C.c_int, restype=C.c_int64)
+_native.register_hip("spmm_token_logprobs", c_vp, C.c_int64, C.c_int64, C.c_int64, C.c_int, c_vp, C.c_int, C.c_int,
+                     C.c_float, C.c_float, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, C.c_int64, c_vp)
+_native.register_hip("spmm_token_logprobs_grad", c_vp, C.c_int64, C.c_int64, C.c_int64, C.c_int, c_vp, C.c_int,
+                     C.c_float, C.c_float, c_vp, c_vp, c_vp, c_vp, c_vp, C.c_int64, c_vp)
+
+MAX_TOP = 128   # vocab_logits.hip kMaxTop
+LOG2E = 1.0 / math.log(2.0)
+
+
+@dataclass
+class TokenLogprobs:
+    logprob: torch.Tensor    # fp32 [n]
+    entropy: torch.Tensor    # fp32 [n]
+    stat: torch.Tensor       # fp32 [n, 2]: the row's maximum m and sum of exp((z - m) / T)
+    temperature: float
+    top: Optional[CSR]       # n x V, k entries a row, largest first (fp32 log-probabilities)
+
+
+def logits_rows(logits: torch.Tensor) -> torch.Tensor:
+    z = R.matrix(logits, "logits")
+    if z.shape[1] < 1 or z.shape[1] >= 2 ** 31 - 4096:
+        raise ValueError(f"a vocabulary has 1 to 2^31 - 4097 columns, got {z.shape[1]}")
+    return z
+
+
+def gradient_out(out: Optional[torch.Tensor], z: torch.Tensor) -> torch.Tensor:
+    """A new gradient of z's shape and type, or the caller's (z itself allowed)."""
+    if out is None:
+        return torch.empty(z.shape, dtype=z.dtype, device=z.device)
+    R.output(out, z.shape, z.dtype, z.device)
+    R.apart(out, z, "logits", in_place=True)
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
+                   temperature: float = 1.0) -> TokenLogprobs:
+    """Log-probability of ``tokens[i]`` (int32 or int64, [n]) in row i of
+    ``logits`` ([n, V] fp32, bf16 or fp16, rows at any stride), the row's
+    entropy, and its ``k`` (at most 128 and at most V; 0: none) largest logits."""
+    R.no_grad_of("token_logprobs_grad", logits)
+    z = logits_rows(logits)
+    n, V = z.shape
+    dev = z.device
+    R.same_device(dev, tokens=tokens)
+    if tokens.dim() != 1 or tokens.shape[0] != n:
+        raise ValueError(f"tokens must be [{n}], got {tuple(tokens.shape)}")
+    tok = R.token_ids(tokens)
+    inv_t = R.inverse_temperature(temperature)
+    k = int(k)
+    if not 0 <= k <= min(MAX_TOP, V):
+        raise ValueError(f"k must be between 0 and {min(MAX_TOP, V)}, got {k}")
+    logprob = torch.empty(n, dtype=torch.float32, device=dev)
+    entropy = torch.empty(n, dtype=torch.float32, device=dev)
+    stat = torch.empty((n, 2), dtype=torch.float32, device=dev)
+    top = None
+    if k:
+        top = CSR(n, V, torch.empty(n + 1, dtype=torch.int64, device=dev),
+                  torch.empty(n * k, dtype=torch.int32, device=dev),
+                  torch.empty(n * k, dtype=torch.float32, device=dev))
+        if n == 0 or dev.type != "cuda":
+            top.rowptr.copy_(torch.arange(0, n * k + 1, k))
+    res = TokenLogprobs(logprob, entropy, stat, float(temperature), top)
+    if n == 0:
+        return res
+    P = _native.ptr
+    if dev.type != "cuda":
+        zf, t = z.float().contiguous(), tok.to(torch.int64)
+        _native.check(_native.host().spmm_cpu_token_logprobs(
+            n, V, P(zf), P(t), inv_t, k, P(logprob), P(entropy), P(stat), P(top.col) if k else None,
+            P(top.val) if k else None, 0), "cpu_token_logprobs")
+        return res
+    lib = _native.hip()
+    code = R.TYPES[z.dtype]
+    bytes_ = lib.spmm_vocab_ws(n, V, code, k)
+    with R.on(dev):
+        ws = torch.empty(bytes_, dtype=torch.uint8, device=dev)
+        _native.check(lib.spmm_token_logprobs(
+            P(z), z.stride(0), n, V, code, P(tok), tok.dtype == torch.int64, k, LOG2E * inv_t, inv_t, P(logprob),
+            P(entropy), P(stat), P(top.rowptr) if k else None, P(top.col) if k else None, P(top.val) if k else None,
+            P(ws), bytes_, _native.stream_ptr(dev)), "token_logprobs")
+    return res
+
+
+def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: TokenLogprobs,
+                        g_logprob: Optional[torch.Tensor] = None, g_entropy: Optional[torch.Tensor] = None,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient with respect to the logits of ``sum_i g_logprob[i] logprob[i] +
+    g_entropy[i] entropy[i]`` (fp32 [n], either may be absent), of the logits'
+    shape and type.  ``stats``: what :func:`token_logprobs` returned for the
+    same logits and tokens.  ``out`` may be the logits themselves.  A row with
+    neither a log-probability's nor an entropy's gradient is zero and its
+    logits are not read."""
+    R.no_grad_of("token_logprobs_grad", logits, g_logprob, g_entropy, out)
+    z = logits_rows(logits)
+    n, V = z.shape
+    dev = z.device
+    R.same_device(dev, tokens=tokens, g_logprob=g_logprob, g_entropy=g_entropy, stats=stats.stat)
+    if tokens.dim() != 1 or tokens.shape[0] != n:
+        raise ValueError(f"tokens must be [{n}], got {tuple(tokens.shape)}")
+    if stats.stat.shape[0] != n:
+        raise ValueError(f"stats are of {stats.stat.shape[0]} rows, the logits have {n}")
+    tok = R.token_ids(tokens)
+    g, h = R.per_row(g_logprob, n, "g_logprob"), R.per_row(g_entropy, n, "g_entropy")
+    inv_t = R.inverse_temperature(stats.temperature)
+    out = gradient_out(out, z)
+    if n == 0:
+        return out
+    P = _native.ptr
+    if dev.type != "cuda":
+        zf, t = z.float().contiguous(), tok.to(torch.int64)
+        acc = torch.empty((n, V), dtype=torch.float32)
+        _native.check(_native.host().spmm_cpu_token_logprobs_grad(n, V, P(zf), P(t), inv_t, P(stats.entropy), P(g),
+                                                                  P(h), P(acc), 0), "cpu_token_logprobs_grad")
+        out.copy_(acc)
+        return out
+    with R.on(dev):
+        _native.check(_native.hip().spmm_token_logprobs_grad(
+            P(z), z.stride(0), n, V, R.TYPES[z.dtype], P(tok), tok.dtype == torch.int64, LOG2E * inv_t, inv_t,
+            P(stats.stat), P(stats.entropy), P(g), P(h), P(out), out.stride(0), _native.stream_ptr(dev)),
+            "token_logprobs_grad")
+    return out
