@@ -93,7 +93,7 @@ SPMM_HOST_EXPORT int spmm_cpu_embedding_grad(int64_t n, int64_t V, int64_t D, co
   return 0;
 }
 
-// stat: [n][2] maximum, Z.  top_col / top_val: [n][k].
+// stat: [2][n] maximum, Z.  top_col / top_val: [n][k].
 SPMM_HOST_EXPORT int spmm_cpu_token_logprobs(int64_t n, int64_t V, const float* z, const int64_t* tok, double inv_t,
                                              int k, float* logprob, float* entropy, float* stat, int32_t* top_col,
                                              float* top_val, int nthreads) {
@@ -108,8 +108,8 @@ SPMM_HOST_EXPORT int spmm_cpu_token_logprobs(int64_t n, int64_t V, const float* 
       const int64_t t = tok[i];
       logprob[i] = t >= 0 && t < V ? (float)((zi[t] - o) * inv_t - logz) : (t == -1 ? 0.f : kNan);
       entropy[i] = r.z == 0 ? 0.f : (float)(logz - r.u / r.z);
-      stat[2 * i] = (float)r.m;
-      stat[2 * i + 1] = (float)r.z;
+      stat[i] = (float)r.m;
+      stat[n + i] = (float)r.z;
       if (k > 0) {
         std::iota(idx.begin(), idx.end(), 0);
         std::partial_sort(idx.begin(), idx.begin() + k, idx.end(),

@@ -84,56 +84,82 @@ __device__ __forceinline__ uint32_t key_of(const void* tok, int wide, int64_t i,
 }
 
 // Few tokens: every token's place is the number of tokens before it, counted
-// against all others.  n^2 compares, one launch: at 8192 tokens as long as
-// the radix passes' launches, less below.
-constexpr int kRankMax = 8192;
-constexpr int kRankTile = 2048;
+// against all others by the 16 waves of a workgroup for its 64 tokens.  One
+// launch and n^2 compares: 5 us at 777 tokens, 15 at 8192, 25 at 16384, where
+// the radix passes' four launches take 22.
+constexpr int kRankMax = 12288;
+constexpr int kRankTile = 4096;   // keys in LDS
+constexpr int kRankWaves = 16;
 
-__global__ __launch_bounds__(256) void embed_rank_sort(const void* __restrict__ tok, int wide, int n, int64_t V,
-                                                       uint32_t* __restrict__ skey, int32_t* __restrict__ spos) {
-  __shared__ uint32_t keys[kRankTile];
-  __shared__ int part[4][64];
+__global__ __launch_bounds__(64 * kRankWaves) void embed_rank_sort(const void* __restrict__ tok, int wide, int n,
+                                                                   int64_t V, uint32_t* __restrict__ skey,
+                                                                   int32_t* __restrict__ spos) {
+  __shared__ __attribute__((aligned(16))) uint32_t keys[kRankTile];
+  __shared__ int part[kRankWaves][64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int i = blockIdx.x * 64 + lane;   // the wave's quarter of every tile against the workgroup's 64 tokens
+  const int i = blockIdx.x * 64 + lane;
   const uint32_t mine = i < n ? key_of(tok, wide, i, V) : 0u;
   int before = 0;
   for (int base = 0; base < n; base += kRankTile) {
+    const int held = n - base < kRankTile ? n - base : kRankTile, blocks = (held + 63) / 64;
     __syncthreads();
-    for (int j = tid; j < kRankTile; j += 256) keys[j] = base + j < n ? key_of(tok, wide, base + j, V) : ~0u;
+    for (int j = tid; j < blocks * 64; j += 64 * kRankWaves) keys[j] = j < held ? key_of(tok, wide, base + j, V) : ~0u;
     __syncthreads();
-    const int j0 = w * (kRankTile / 4);
-    const int left = n - base - j0, count = left < kRankTile / 4 ? left : kRankTile / 4;
-    // equal keys keep their order: those at lower positions count as before
-    for (int j = 0; j < count; ++j) {
-      const uint32_t k = keys[j0 + j];
-      before += (k < mine || (k == mine && base + j0 + j < i)) ? 1 : 0;
+    for (int b = w; b < blocks; b += kRankWaves) {
+      const u32x4* k4 = reinterpret_cast<const u32x4*>(keys + b * 64);
+      const int own = (int)blockIdx.x - base / 64;   // the workgroup's own tokens are that block
+      // equal keys keep their order: those of earlier blocks are before, of later ones behind
+      if (b < own) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const u32x4 k = k4[q];
+          before += (k[0] <= mine) + (k[1] <= mine) + (k[2] <= mine) + (k[3] <= mine);
+        }
+      } else if (b > own) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const u32x4 k = k4[q];
+          before += (k[0] < mine) + (k[1] < mine) + (k[2] < mine) + (k[3] < mine);
+        }
+      } else {
+#pragma unroll 4
+        for (int q = 0; q < 64; ++q) {
+          const uint32_t k = keys[b * 64 + q];
+          before += (k < mine || (k == mine && q < lane)) ? 1 : 0;
+        }
+      }
     }
   }
   part[w][lane] = before;
   __syncthreads();
   if (w == 0 && i < n) {
-    const int at = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+    int at = 0;
+#pragma unroll
+    for (int q = 0; q < kRankWaves; ++q) at += part[q][lane];
     skey[at] = mine;
     spos[at] = i;
   }
 }
 
 // Many tokens: least-significant-digit radix sort, digits of up to 10 bits.
-// A wave ranks 16 rounds of 64 keys in order against its own digit counters
-// (no workgroup barrier inside), equal digits of a round by ballots.
-constexpr int kRounds = 16;
-constexpr int kSortTile = 256 * kRounds;   // keys a workgroup
+// A wave ranks its rounds of 64 keys in order against its own digit counters
+// (no workgroup barrier inside), equal digits of a round by ballots.  With few
+// tiles every scatter workgroup adds up the counters in front of it by itself;
+// with many a scan of its own does it once.
 constexpr int kMaxBits = 10;
+constexpr int kSmallRounds = 4, kLargeRounds = 16;   // keys a wave / 64
+constexpr int64_t kFewTiles = 128;
 
 __global__ __launch_bounds__(256) void embed_digit_count(const void* __restrict__ tok, int wide,
                                                          const uint32_t* __restrict__ key, int64_t n, int64_t V,
-                                                         int shift, int bits, int64_t tiles, int32_t* __restrict__ cnt) {
+                                                         int shift, int bits, int rounds, int32_t* __restrict__ cnt) {
   __shared__ int h[1 << kMaxBits];
   const int bins = 1 << bits;
   for (int b = threadIdx.x; b < bins; b += 256) h[b] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kSortTile;
-  for (int r = 0; r < kRounds; ++r) {
+  const int64_t base = (int64_t)blockIdx.x * 256 * rounds;
+#pragma unroll 4
+  for (int r = 0; r < rounds; ++r) {
     const int64_t i = base + r * 256 + threadIdx.x;
     if (i < n) {
       const uint32_t k = key ? key[i] : key_of(tok, wide, i, V);
@@ -141,70 +167,121 @@ __global__ __launch_bounds__(256) void embed_digit_count(const void* __restrict_
     }
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += 256) cnt[(int64_t)b * tiles + blockIdx.x] = h[b];
+  for (int b = threadIdx.x; b < bins; b += 256) cnt[((int64_t)blockIdx.x << bits) + b] = h[b];
 }
 
-// exclusive scan of the (digit, tile) counters, one workgroup
-__global__ __launch_bounds__(1024) void embed_digit_scan(int32_t* __restrict__ cnt, int64_t m) {
-  __shared__ int wsum[16];
-  __shared__ int carry;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  if (tid == 0) carry = 0;
-  for (int64_t base = 0; base < m; base += 1024 * 8) {
-    int v[8], s = 0;
+// Where each digit of a tile starts among all keys, from the tiles' counters
+// [tile][digit]: keys of smaller digits, then those of this digit in the tiles
+// in front.  One workgroup of 256 threads; start[] in LDS.
+template <int PER>   // consecutive digits a thread
+__device__ __forceinline__ void digit_starts(const int32_t* __restrict__ cnt, int64_t tiles, int64_t tile, int bits,
+                                             int* start, int* wsum) {
+  constexpr int kLoads = 16;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, bins = 1 << bits;
+  const int first = tid * PER < bins ? tid * PER : 0;
+  int front[PER] = {}, total[PER] = {};
+  for (int64_t t0 = 0; t0 < tiles; t0 += kLoads) {
+    int c[kLoads][PER];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int64_t i = base + (int64_t)tid * 8 + u;
-      v[u] = i < m ? cnt[i] : 0;
-      s += v[u];
-    }
-    int incl = s;
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t t = t0 + u < tiles ? t0 + u : tiles - 1;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int y = __shfl_up(incl, d);
-      if (lane >= d) incl += y;
+      for (int q = 0; q < PER; ++q) c[u][q] = cnt[(t << bits) + first + q];
     }
-    if (lane == 63) wsum[w] = incl;
-    __syncthreads();
-    int pre = carry, tot = 0;
-    for (int q = 0; q < 16; ++q) {
-      pre += q < w ? wsum[q] : 0;
-      tot += wsum[q];
-    }
-    int run = pre + incl - s;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int64_t i = base + (int64_t)tid * 8 + u;
-      if (i < m) cnt[i] = run;
-      run += v[u];
+    for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+      for (int q = 0; q < PER; ++q) {
+        const int x = t0 + u < tiles ? c[u][q] : 0;
+        total[q] += x;
+        front[q] += t0 + u < tile ? x : 0;
+      }
+  }
+  int s = 0;
+#pragma unroll
+  for (int q = 0; q < PER; ++q) s += tid * PER < bins ? total[q] : 0;
+  int incl = s;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(incl, d);
+    if (lane >= d) incl += y;
+  }
+  if (lane == 63) wsum[w] = incl;
+  __syncthreads();
+  int run = incl - s;
+  for (int q = 0; q < w; ++q) run += wsum[q];
+  if (tid * PER < bins) {
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      start[tid * PER + q] = run + front[q];
+      run += total[q];
     }
-    __syncthreads();   // every read of carry and wsum done
-    if (tid == 0) carry += tot;
-    __syncthreads();
   }
 }
 
+// The same for many tiles, once a pass: cnt becomes the starts.  Digit by
+// digit over the tiles, then over the digits' totals; one workgroup.
+__global__ __launch_bounds__(1024) void embed_digit_scan(int32_t* __restrict__ cnt, int64_t tiles, int bits) {
+  __shared__ int wsum[16];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, bins = 1 << bits;
+  int total = 0;
+  if (tid < bins)
+    for (int64_t t0 = 0; t0 < tiles; t0 += 16) {
+      int c[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) c[u] = t0 + u < tiles ? cnt[((t0 + u) << bits) + tid] : 0;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) total += c[u];
+    }
+  int incl = total;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(incl, d);
+    if (lane >= d) incl += y;
+  }
+  if (lane == 63) wsum[w] = incl;
+  __syncthreads();
+  int run = incl - total;
+  for (int q = 0; q < w; ++q) run += wsum[q];
+  if (tid < bins)
+    for (int64_t t0 = 0; t0 < tiles; t0 += 16) {
+      int c[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) c[u] = t0 + u < tiles ? cnt[((t0 + u) << bits) + tid] : 0;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        if (t0 + u < tiles) cnt[((t0 + u) << bits) + tid] = run;
+        run += c[u];
+      }
+    }
+}
+
+template <int R>
 __global__ __launch_bounds__(256) void embed_digit_scatter(const void* __restrict__ tok, int wide,
                                                            const uint32_t* __restrict__ kin,
                                                            const int32_t* __restrict__ pin, int64_t n, int64_t V,
-                                                           int shift, int bits, int64_t tiles,
-                                                           const int32_t* __restrict__ offs, uint32_t* __restrict__ kout,
+                                                           int shift, int bits, int64_t tiles, int scanned,
+                                                           const int32_t* __restrict__ cnt, uint32_t* __restrict__ kout,
                                                            int32_t* __restrict__ pout) {
   __shared__ int wcnt[4][1 << kMaxBits];
+  __shared__ int start[1 << kMaxBits];
+  __shared__ int wsum[4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, bins = 1 << bits;
   for (int b = tid; b < bins; b += 256) wcnt[0][b] = wcnt[1][b] = wcnt[2][b] = wcnt[3][b] = 0;
-  __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kSortTile + (int64_t)w * (64 * kRounds);
+  const int64_t base = (int64_t)blockIdx.x * (256 * R) + (int64_t)w * (64 * R);
   const unsigned long long below = (1ull << lane) - 1ull;
-  uint32_t k[kRounds];
-  int rank[kRounds];
+  uint32_t k[R];
+  int32_t pos[R];
+  int rank[R];
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
+  for (int r = 0; r < R; ++r) {
     const int64_t i = base + r * 64 + lane;
     k[r] = i < n ? (kin ? kin[i] : key_of(tok, wide, i, V)) : 0u;
+    pos[r] = i < n ? (pin ? pin[i] : (int32_t)i) : 0;
   }
+  __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
+  for (int r = 0; r < R; ++r) {
     const bool ok = base + r * 64 + lane < n;
     const int d = (int)(k[r] >> shift) & (bins - 1);
     unsigned long long m = __ballot(ok);
@@ -221,77 +298,100 @@ __global__ __launch_bounds__(256) void embed_digit_scatter(const void* __restric
     if (ok && in_round == 0) wcnt[w][d] = seen + __popcll(m);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
+  if (scanned) {
+    for (int b = tid; b < bins; b += 256) start[b] = cnt[((int64_t)blockIdx.x << bits) + b];
+  } else {
+    if (bits <= 8) digit_starts<1>(cnt, tiles, blockIdx.x, bits, start, wsum);
+    else if (bits == 9) digit_starts<2>(cnt, tiles, blockIdx.x, bits, start, wsum);
+    else digit_starts<4>(cnt, tiles, blockIdx.x, bits, start, wsum);
+  }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = base + r * 64 + lane;
-    if (i >= n) continue;
+  for (int r = 0; r < R; ++r) {
+    if (base + r * 64 + lane >= n) continue;
     const int d = (int)(k[r] >> shift) & (bins - 1);
-    int at = offs[(int64_t)d * tiles + blockIdx.x] + rank[r];
+    int at = start[d] + rank[r];
     for (int q = 0; q < w; ++q) at += wcnt[q][d];
     kout[at] = k[r];
-    pout[at] = pin ? pin[i] : (int32_t)i;
+    pout[at] = pos[r];
   }
 }
 
 // ---- sums ---------------------------------------------------------------------
+// tile: sorted entries a wave of embed_grad_sum
 struct GradArgs {
   const void* dy;
   int64_t lddy;
   const uint32_t* skey;
   const int32_t* spos;
-  int64_t n, V, D, ldw, tiles, slices, vblocks;
+  int64_t n, V, D, ldw, tile, tiles, slices, vblocks;
   float scale;
   void* dw;
   float* part;   // [tiles][2][D]: a tile's sums of the run it begins inside and of the one it ends inside
   int accumulate;
 };
 
-constexpr int kTile = 32;       // sorted entries a wave
+// Sorted entries a wave sums: 8 in a short batch, which has few waves to hide
+// their loads behind; 32 else, which writes a quarter of the partial rows.
+constexpr int64_t kShortBatch = 2048;
 constexpr int kFlight = 8;      // row loads in flight
-constexpr int kFillRows = 16;   // table rows a zero-filling wave
+constexpr int kFillRows = 32;   // table rows a zero-filling wave
 
-// N floats of columns [c, c + N) (fewer at the row's end), from / to a row of any of the types
-template <typename T, int N>
-__device__ __forceinline__ void load_cols(const T* row, int64_t c, int64_t D, float (&x)[N]) {
-  if (c + N <= D) {
-#pragma unroll
-    for (int b = 0; b < N; b += Elem<T>::kN) {
-      const u32x4 r = load_vec(row + c + b);
-#pragma unroll
-      for (int e = 0; e < Elem<T>::kN; ++e) x[b + e] = Elem<T>::get(r, e);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = c + e < D ? Elem<T>::load(row + c + e) : 0.f;
+// The first of the sorted keys at or behind lo that is not before v: 64 probes a step.
+__device__ __forceinline__ int64_t first_not_before(const uint32_t* __restrict__ skey, int64_t lo, int64_t n, int64_t v) {
+  const int lane = threadIdx.x & 63;
+  int64_t hi = n;
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 63) / 64, i = lo + lane * step;
+    const int c = __popcll(__ballot(i < hi && (int64_t)skey[i] < v));   // the probes before v are the first ones
+    if (c == 0) return lo;
+    const int64_t end = lo + c * step;
+    lo += (c - 1) * step + 1;
+    hi = end < hi ? end : hi;
   }
+  return lo;
 }
 
+// Columns [c, c + N) of a row of any of the types.  A row's last lane reaches
+// back (`from` = D - N < c) so that every lane reads whole vectors; what it
+// reads of its neighbour's columns is summed and not written.
 template <typename T, int N>
-__device__ __forceinline__ void store_cols(T* row, int64_t c, int64_t D, const float (&x)[N]) {
-  if (c + N <= D) {
+struct Cols {
+  static constexpr int kVecs = N / Elem<T>::kN > 0 ? N / Elem<T>::kN : 1;
+  u32x4 v[kVecs];
+  __device__ __forceinline__ void load(const T* row, int64_t from) {
+#pragma unroll
+    for (int b = 0; b < kVecs; ++b) v[b] = load_vec(row + from + b * Elem<T>::kN);
+  }
+  __device__ __forceinline__ float get(int e) const { return Elem<T>::get(v[e / Elem<T>::kN], e % Elem<T>::kN); }
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void store_cols(T* row, int64_t c, int64_t from, const float (&x)[N]) {
+  if (from == c) {
 #pragma unroll
     for (int b = 0; b < N; b += Elem<T>::kN) store_vec(row + c + b, Elem<T>::pack(x + b));
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (c + e < D) row[c + e] = Elem<T>::cast(x[e]);
+      if (from + e >= c) row[from + e] = Elem<T>::cast(x[e]);
   }
 }
 
 // the finished fp32 sum of one token's row: scaled, added to what is there, rounded once
 template <typename TO, int N>
-__device__ __forceinline__ void finish_row(const GradArgs& a, int64_t v, int64_t c, float (&acc)[N]) {
+__device__ __forceinline__ void finish_row(const GradArgs& a, int64_t v, int64_t c, int64_t from, float (&acc)[N]) {
   TO* row = static_cast<TO*>(a.dw) + v * a.ldw;
-#pragma unroll
-  for (int e = 0; e < N; ++e) acc[e] *= a.scale;
   if (a.accumulate) {
-    float old[N];
-    load_cols<TO, N>(row, c, a.D, old);
+    Cols<TO, N> old;
+    old.load(row, from);
 #pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] += old[e];
+    for (int e = 0; e < N; ++e) acc[e] = __builtin_fmaf(acc[e], a.scale, old.get(e));
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] *= a.scale;
   }
-  store_cols<TO, N>(row, c, a.D, acc);
+  store_cols<TO, N>(row, c, from, acc);
 }
 
 template <typename TI, typename TO>
@@ -303,28 +403,29 @@ __global__ __launch_bounds__(256) void embed_grad_sum(GradArgs a) {
   for (int64_t t = wave; t < tasks; t += waves) {
     if (t >= sums) {   // zero rows for tokens that the batch does not have
       const int64_t v0 = (t - sums) * kFillRows;
-      // lane r finds where row v0 + r would start among the sorted keys
-      int64_t lo = 0, hi = a.n;
-      const int64_t v = v0 + (lane < kFillRows ? lane : kFillRows - 1);
+      int64_t lo = first_not_before(a.skey, 0, a.n, v0), hi = first_not_before(a.skey, lo, a.n, v0 + kFillRows);
+      const int64_t v = v0 + lane, end = hi;   // lane r finds its row between them
       while (lo < hi) {
         const int64_t mid = (lo + hi) >> 1;
         if ((int64_t)a.skey[mid] < v) lo = mid + 1; else hi = mid;
       }
-      const bool empty = v < a.V && (lo >= a.n || (int64_t)a.skey[lo] != v);
+      const bool empty = lane < kFillRows && v < a.V && (lo >= end || (int64_t)a.skey[lo] != v);
       const unsigned long long m = __ballot(empty);
       constexpr int NO = Elem<TO>::kN;
-      const float zero[NO] = {};
+      const int64_t nv = a.D / NO;
       for (int r = 0; r < kFillRows; ++r) {
         if (!((m >> r) & 1)) continue;
         TO* row = static_cast<TO*>(a.dw) + (v0 + r) * a.ldw;
-        for (int64_t c = (int64_t)lane * NO; c < a.D; c += 64 * NO) store_cols<TO, NO>(row, c, a.D, zero);
+        for (int64_t i = lane; i < nv; i += 64) store_vec(row + i * NO, u32x4{0u, 0u, 0u, 0u});
+        if (nv * NO + lane < a.D) row[nv * NO + lane] = Elem<TO>::cast(0.f);
       }
       continue;
     }
     const int64_t tile = t / a.slices, c = ((t - tile * a.slices) * 64 + lane) * N;
-    const int64_t b = tile * kTile, e = b + kTile < a.n ? b + kTile : a.n;
+    const int64_t b = tile * a.tile, e = b + a.tile < a.n ? b + a.tile : a.n;
     const bool mine = c < a.D;
-    // the tile's tokens and positions, one a lane (a padded lane repeats the last)
+    const int64_t from = c + N <= a.D ? c : a.D - N;   // (D >= N)
+    // the tile's tokens and positions, one a lane (further lanes repeat the last)
     const int64_t at = b + lane < e ? b + lane : e - 1;
     const int key = (int)a.skey[at], pos = a.spos[at];
     const int V = (int)a.V;
@@ -332,15 +433,12 @@ __global__ __launch_bounds__(256) void embed_grad_sum(GradArgs a) {
     const int cnt = (int)(e - b);
     float acc[N] = {};
     bool head = true;   // the current run reaches back to the tile's first entry
-    for (int r0 = 0; r0 < cnt; r0 += kFlight) {
-      float x[kFlight][N];
+    for (int r0 = 0; r0 < cnt && __builtin_amdgcn_readlane(key, r0) < V; r0 += kFlight) {
+      Cols<TI, N> x[kFlight];
 #pragma unroll
-      for (int u = 0; u < kFlight; ++u) {
-        const int r = r0 + u < cnt ? r0 + u : cnt - 1;
-        const int64_t p = __builtin_amdgcn_readlane(pos, r);
-        if (mine && __builtin_amdgcn_readlane(key, r) < V)
-          load_cols<TI, N>(static_cast<const TI*>(a.dy) + p * a.lddy, c, a.D, x[u]);
-      }
+      for (int u = 0; u < kFlight; ++u)   // (behind the last entry: that one again)
+        x[u].load(static_cast<const TI*>(a.dy) + (int64_t)__builtin_amdgcn_readlane(pos, r0 + u < cnt ? r0 + u : cnt - 1) * a.lddy,
+                  from);
 #pragma unroll
       for (int u = 0; u < kFlight; ++u) {
         const int r = r0 + u;
@@ -349,15 +447,14 @@ __global__ __launch_bounds__(256) void embed_grad_sum(GradArgs a) {
         if (kr >= V) break;   // padding: nothing behind it either
         const int next = r + 1 < cnt ? __builtin_amdgcn_readlane(key, r + 1) : after;
 #pragma unroll
-        for (int q = 0; q < N; ++q) acc[q] += x[u][q];
+        for (int q = 0; q < N; ++q) acc[q] += x[u].get(q);
         if (next == kr && r + 1 < cnt) continue;
         const bool from_before = head && before == kr, into_next = r + 1 == cnt && after == kr;
         if (mine) {
           if (!from_before && !into_next) {
-            finish_row<TO, N>(a, kr, c, acc);
+            finish_row<TO, N>(a, kr, c, from, acc);
           } else {   // slot 0: a run that began in an earlier tile; slot 1: one that goes on from here
-            float* p = a.part + (tile * 2 + (from_before ? 0 : 1)) * a.D;
-            store_cols<float, N>(p, c, a.D, acc);
+            store_cols<float, N>(a.part + (tile * 2 + (from_before ? 0 : 1)) * a.D, c, from, acc);
           }
         }
 #pragma unroll
@@ -368,104 +465,145 @@ __global__ __launch_bounds__(256) void embed_grad_sum(GradArgs a) {
   }
 }
 
-// Runs that cross tiles: the tile where a run begins adds its own partial row
-// and those of the tiles that the run goes through, in order.  Four waves take
-// a quarter of the tiles each.
+// Rows narrower than a vector: a thread a table row's column, from the sorted entries.
 template <typename TI, typename TO>
-__global__ __launch_bounds__(256) void embed_grad_join(GradArgs a) {
-  constexpr int N = 4;   // columns a lane: partial rows are fp32
-  __shared__ float sums[3][64 * N];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t slices = (a.D + 64 * N - 1) / (64 * N), tasks = a.tiles * slices;
-  for (int64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
-    const int64_t tile = t / slices, c = ((t - tile * slices) * 64 + lane) * N;
-    const int64_t b = tile * kTile, e = b + kTile;
-    if (e >= a.n) continue;   // (uniform) nothing follows the last tile
-    const uint32_t key = a.skey[e - 1];
-    if (key >= (uint32_t)a.V || a.skey[e] != key) continue;          // no run crosses here
-    if (a.skey[b] == key && b > 0 && a.skey[b - 1] == key) continue; // it began in an earlier tile
-    // the last tile that the run reaches
-    int64_t lo = e, hi = a.n;   // first entry behind the run
+__global__ __launch_bounds__(256) void embed_grad_narrow(GradArgs a) {
+  const int64_t tasks = a.V * a.D;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < tasks; t += (int64_t)gridDim.x * 256) {
+    const int64_t v = t / a.D, c = t - v * a.D;
+    int64_t lo = 0, hi = a.n;
     while (lo < hi) {
       const int64_t mid = (lo + hi) >> 1;
-      if (a.skey[mid] <= key) lo = mid + 1; else hi = mid;
+      if ((int64_t)a.skey[mid] < v) lo = mid + 1; else hi = mid;
     }
-    const int64_t last = (lo - 1) / kTile, m = last - tile + 1;   // partial rows: this tile's and those behind it
-    const int64_t q0 = m * w / 4, q1 = m * (w + 1) / 4;
-    float acc[N] = {};
-    for (int64_t q = q0; q < q1; q += kFlight) {
-      float x[kFlight][N];
+    const bool any = lo < a.n && (int64_t)a.skey[lo] == v;
+    if (a.accumulate && !any) continue;
+    float acc = 0.f;
+    for (; lo < a.n && (int64_t)a.skey[lo] == v; ++lo)
+      acc += Elem<TI>::load(static_cast<const TI*>(a.dy) + (int64_t)a.spos[lo] * a.lddy + c);
+    TO* out = static_cast<TO*>(a.dw) + v * a.ldw + c;
+    *out = Elem<TO>::cast(a.accumulate ? __builtin_fmaf(acc, a.scale, Elem<TO>::load(out)) : acc * a.scale);
+  }
+}
+
+// Runs that cross tiles: the tile where a run begins adds its own partial row
+// and those of the tiles that the run goes through, in order.  A wave looks at
+// one tile and adds up to kFlight rows by itself; the waves of a workgroup
+// share the longer runs that they found.
+constexpr int kJoinWaves = 8;
+
+// rows q0 .. q1 of a run that begins in `tile`
+template <int N>
+__device__ __forceinline__ void add_parts(const GradArgs& a, int64_t tile, int64_t q0, int64_t q1, int64_t from,
+                                          float (&acc)[N]) {
+  for (int64_t q = q0; q < q1; q += kFlight) {
+    Cols<float, N> x[kFlight];
 #pragma unroll
-      for (int u = 0; u < kFlight; ++u) {
-        const int64_t i = q + u < q1 ? q + u : q1 - 1;
-        if (c < a.D) load_cols<float, N>(a.part + ((tile + i) * 2 + (i == 0 ? 1 : 0)) * a.D, c, a.D, x[u]);
-      }
+    for (int u = 0; u < kFlight; ++u) {
+      const int64_t i = q + u < q1 ? q + u : q1 - 1;
+      x[u].load(a.part + ((tile + i) * 2 + (i == 0 ? 1 : 0)) * a.D, from);
+    }
 #pragma unroll
-      for (int u = 0; u < kFlight; ++u)
-        if (q + u < q1) {
+    for (int u = 0; u < kFlight; ++u) {
+      if (q + u >= q1) break;
 #pragma unroll
-          for (int s = 0; s < N; ++s) acc[s] += x[u][s];
+      for (int s = 0; s < N; ++s) acc[s] += x[u].get(s);
+    }
+  }
+}
+
+template <typename TI, typename TO>
+__global__ __launch_bounds__(64 * kJoinWaves) void embed_grad_join(GradArgs a) {
+  constexpr int N = Elem<TO>::kN;   // columns a lane
+  __shared__ float sums[kJoinWaves - 1][64 * N];
+  __shared__ int64_t rows[kJoinWaves];   // partial rows of the waves' longer runs, 0: none
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t slices = (a.D + 64 * N - 1) / (64 * N), tasks = a.tiles * slices;
+  // a workgroup's waves take tasks far apart: a long run's slices go to as many workgroups
+  const int64_t groups = (tasks + kJoinWaves - 1) / kJoinWaves;
+  for (int64_t t0 = blockIdx.x; t0 < groups; t0 += gridDim.x) {
+    int64_t m = 0;
+    const int64_t t = t0 + w * groups, tile = t / slices, b = tile * a.tile, e = b + a.tile;
+    if (t < tasks && e < a.n) {   // (nothing follows the last tile)
+      const uint32_t key = a.skey[e - 1], next = a.skey[e], first = a.skey[b], front = b > 0 ? a.skey[b - 1] : ~0u;
+      // a run crosses here, and it did not begin in an earlier tile
+      if (key < (uint32_t)a.V && next == key && !(first == key && front == key)) {
+        m = (first_not_before(a.skey, e, a.n, (int64_t)key + 1) - 1) / a.tile - tile + 1;
+        if (m <= kFlight) {
+          const int64_t c = ((t - tile * slices) * 64 + lane) * N, from = c + N <= a.D ? c : a.D - N;
+          float acc[N] = {};
+          add_parts<N>(a, tile, 0, m, from, acc);
+          if (c < a.D) finish_row<TO, N>(a, key, c, from, acc);
+          m = 0;
         }
-    }
-    __syncthreads();
-    if (w > 0) {
-#pragma unroll
-      for (int s = 0; s < N; ++s) sums[w - 1][lane * N + s] = acc[s];
-    }
-    __syncthreads();
-    if (w == 0 && c < a.D) {
-#pragma unroll
-      for (int q = 0; q < 3; ++q)
-#pragma unroll
-        for (int s = 0; s < N; ++s) acc[s] += sums[q][lane * N + s];
-      if constexpr (Elem<TO>::kN == N) {
-        finish_row<TO, N>(a, key, c, acc);
-      } else {   // 16-bit outputs: four columns are half a vector
-        TO* row = static_cast<TO*>(a.dw) + (int64_t)key * a.ldw;
-#pragma unroll
-        for (int s = 0; s < N; ++s) {
-          if (c + s >= a.D) break;
-          float x = acc[s] * a.scale;
-          if (a.accumulate) x += Elem<TO>::load(row + c + s);
-          row[c + s] = Elem<TO>::cast(x);
-        }
       }
+    }
+    __syncthreads();   // the last round's rows and sums are read
+    if (lane == 0) rows[w] = m;
+    __syncthreads();
+    for (int f = 0; f < kJoinWaves; ++f) {
+      m = rows[f];
+      if (m == 0) continue;   // (uniform)
+      const int64_t t_f = t0 + f * groups, tile_f = t_f / slices;
+      const int64_t c = ((t_f - tile_f * slices) * 64 + lane) * N, from = c + N <= a.D ? c : a.D - N;
+      float acc[N] = {};
+      add_parts<N>(a, tile_f, m * w / kJoinWaves, m * (w + 1) / kJoinWaves, from, acc);
+      if (w > 0) {
+#pragma unroll
+        for (int s = 0; s < N; ++s) sums[w - 1][s * 64 + lane] = acc[s];
+      }
+      __syncthreads();
+      if (w == 0 && c < a.D) {
+#pragma unroll
+        for (int q = 0; q < kJoinWaves - 1; ++q)
+#pragma unroll
+          for (int s = 0; s < N; ++s) acc[s] += sums[q][s * 64 + lane];
+        finish_row<TO, N>(a, a.skey[(tile_f + 1) * a.tile], c, from, acc);
+      }
+      __syncthreads();
     }
   }
 }
 
 struct GradSizes {
-  int64_t tiles, sort_tiles, keys, part, cnt, total;
-  int bits, passes;
+  int64_t tile, tiles, sort_tiles, keys, cnt, total;
+  int bits, passes, rounds;
 };
 
 // Layout of the workspace: sorted keys and positions (twice for the radix
 // passes), digit counters, partial rows.
 bool grad_sizes(int64_t n, int64_t V, int64_t D, GradSizes& g) {
-  if (n < 0 || n >= (1ll << 31) - kSortTile || V < 1 || V >= (1ll << 31) - 1 || D < 1) return false;
+  if (n < 0 || n >= (1ll << 31) - (1 << 20) || V < 1 || V >= (1ll << 31) - 1 || D < 1) return false;
   int total_bits = 1;
   while ((V >> total_bits) != 0) ++total_bits;   // keys 0 .. V
   g.passes = (total_bits + kMaxBits - 1) / kMaxBits;
   g.bits = (total_bits + g.passes - 1) / g.passes;
-  g.tiles = (n + kTile - 1) / kTile;
-  g.sort_tiles = (n + kSortTile - 1) / kSortTile;
+  g.tile = n <= kShortBatch ? 8 : 32;
+  g.tiles = (n + g.tile - 1) / g.tile;
+  g.rounds = n <= kFewTiles * 256 * kSmallRounds ? kSmallRounds : kLargeRounds;
+  g.sort_tiles = (n + 256 * g.rounds - 1) / (256 * g.rounds);
   g.keys = (n + 63) / 64 * 64;
-  g.cnt = n > kRankMax ? ((int64_t)g.sort_tiles << g.bits) : 0;
-  g.part = g.tiles * 2 * D;
+  g.cnt = n > kRankMax ? (g.sort_tiles << g.bits) : 0;
   const int64_t copies = n > kRankMax ? 2 : 1;
-  g.total = (g.keys * 2 * copies + (g.cnt + 63) / 64 * 64) * 4 + g.part * 4;
+  g.total = (g.keys * 2 * copies + (g.cnt + 63) / 64 * 64 + g.tiles * 2 * D) * 4;
   return true;
 }
 
 template <typename TI, typename TO>
 int grad(GradArgs a, hipStream_t s) {
+  if (a.D < 8) {   // (narrower than a vector of the 16-bit types)
+    hipLaunchKernelGGL((embed_grad_narrow<TI, TO>), dim3(groups_of((a.V * a.D + 255) / 256)), dim3(256), 0, s, a);
+    SPMM_LAUNCH_CHECK();
+    return 0;
+  }
   const int64_t waves = a.tiles * a.slices + a.vblocks;
   if (waves > 0)
     hipLaunchKernelGGL((embed_grad_sum<TI, TO>), dim3(groups_of((waves + 3) / 4)), dim3(256), 0, s, a);
   SPMM_LAUNCH_CHECK();
   if (a.tiles > 1) {
-    const int64_t joins = a.tiles * ((a.D + 255) / 256);
-    hipLaunchKernelGGL((embed_grad_join<TI, TO>), dim3(groups_of(joins)), dim3(256), 0, s, a);
+    const int64_t joins = a.tiles * ((a.D + 64 * Elem<TO>::kN - 1) / (64 * Elem<TO>::kN));
+    hipLaunchKernelGGL((embed_grad_join<TI, TO>), dim3(groups_of((joins + kJoinWaves - 1) / kJoinWaves)),
+                       dim3(64 * kJoinWaves), 0, s, a);
     SPMM_LAUNCH_CHECK();
   }
   return 0;
@@ -507,13 +645,18 @@ SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, c
     const int32_t* pin = nullptr;
     uint32_t* kout = ka;
     int32_t* pout = pa;
+    const bool scan = g.sort_tiles > kFewTiles;
     for (int p = 0; p < g.passes; ++p) {
       const int shift = p * g.bits;
-      hipLaunchKernelGGL(embed_digit_count, dim3((unsigned)g.sort_tiles), dim3(256), 0, s, tok, wide, kin, n, V, shift,
-                         g.bits, g.sort_tiles, cnt);
-      hipLaunchKernelGGL(embed_digit_scan, dim3(1), dim3(1024), 0, s, cnt, g.cnt);
-      hipLaunchKernelGGL(embed_digit_scatter, dim3((unsigned)g.sort_tiles), dim3(256), 0, s, tok, wide, kin, pin, n, V,
-                         shift, g.bits, g.sort_tiles, cnt, kout, pout);
+      const dim3 grid((unsigned)g.sort_tiles);
+      hipLaunchKernelGGL(embed_digit_count, grid, dim3(256), 0, s, tok, wide, kin, n, V, shift, g.bits, g.rounds, cnt);
+      if (scan) hipLaunchKernelGGL(embed_digit_scan, dim3(1), dim3(1024), 0, s, cnt, g.sort_tiles, g.bits);
+      if (g.rounds == kSmallRounds)
+        hipLaunchKernelGGL((embed_digit_scatter<kSmallRounds>), grid, dim3(256), 0, s, tok, wide, kin, pin, n, V, shift,
+                           g.bits, g.sort_tiles, (int)scan, cnt, kout, pout);
+      else
+        hipLaunchKernelGGL((embed_digit_scatter<kLargeRounds>), grid, dim3(256), 0, s, tok, wide, kin, pin, n, V, shift,
+                           g.bits, g.sort_tiles, (int)scan, cnt, kout, pout);
       kin = kout;
       pin = pout;
       kout = kout == ka ? kb : ka;
@@ -522,8 +665,8 @@ SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, c
     skey = const_cast<uint32_t*>(kin);
     spos = const_cast<int32_t*>(pin);
   } else if (n > 0) {
-    hipLaunchKernelGGL(embed_rank_sort, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, s, tok, wide, (int)n, V, skey,
-                       spos);
+    hipLaunchKernelGGL(embed_rank_sort, dim3((unsigned)((n + 63) / 64)), dim3(64 * kRankWaves), 0, s, tok, wide, (int)n,
+                       V, skey, spos);
   }
   SPMM_LAUNCH_CHECK();
   GradArgs a;
@@ -535,6 +678,7 @@ SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, c
   a.V = V;
   a.D = D;
   a.ldw = ldw;
+  a.tile = g.tile;
   a.tiles = g.tiles;
   a.vblocks = accumulate ? 0 : (V + kFillRows - 1) / kFillRows;
   a.scale = scale;

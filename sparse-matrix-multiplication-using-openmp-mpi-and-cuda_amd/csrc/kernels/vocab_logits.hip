@@ -310,7 +310,7 @@ struct JoinArgs {
   const void* tok;
   int wide, k;
   const uint64_t* lists;
-  float *logprob, *entropy, *stat;   // stat: [n][2] maximum and Z
+  float *logprob, *entropy, *stat;   // stat: [2][n] maximum and Z
   int64_t* rowptr;
   int32_t* top_col;
   float* top_val;
@@ -338,8 +338,8 @@ __global__ __launch_bounds__(kThreads) void vocab_join(JoinArgs a) {
         lp = __builtin_nanf("");
       a.logprob[row] = lp;
       a.entropy[row] = st.z == 0.f ? 0.f : kLn2 * (l2z - st.u / st.z);
-      a.stat[row * 2] = st.m;
-      a.stat[row * 2 + 1] = st.z;
+      a.stat[row] = st.m;
+      a.stat[a.n + row] = st.z;
     }
     if constexpr (TOP) {
       // every entry's place: how many of the other segments' (descending) lists are above it
@@ -418,8 +418,8 @@ __global__ __launch_bounds__(kThreads) void vocab_token_grad(TokenGradArgs a) {
       continue;
     }
     if (id < -1 || id >= a.V) g = __builtin_nanf("");
-    const float Z = a.stat[row * 2 + 1], l2z = Z == 0.f ? 0.f : __builtin_amdgcn_logf(Z), rz = Z == 0.f ? 0.f : 1.f / Z;
-    const Origin o(a.stat[row * 2], a.c);
+    const float Z = a.stat[a.n + row], l2z = Z == 0.f ? 0.f : __builtin_amdgcn_logf(Z), rz = Z == 0.f ? 0.f : 1.f / Z;
+    const Origin o(a.stat[row], a.c);
     const float beta = -h * kLn2 * rz, alpha = -(g + (ENT ? h * (a.entropy[row] - kLn2 * l2z) : 0.f)) * rz;
     u32x4 r[VPT];
 #pragma unroll

@@ -46,7 +46,7 @@ LOG2E = 1.0 / math.log(2.0)
 class TokenLogprobs:
     logprob: torch.Tensor    # fp32 [n]
     entropy: torch.Tensor    # fp32 [n]
-    stat: torch.Tensor       # fp32 [n, 2]: the row's maximum m and sum of exp((z - m) / T)
+    stat: torch.Tensor       # fp32 [2, n]: the row's maximum m and sum of exp((z - m) / T)
     temperature: float
     top: Optional[CSR]       # n x V, k entries a row, largest first (fp32 log-probabilities)
 
@@ -84,9 +84,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     k = int(k)
     if not 0 <= k <= min(MAX_TOP, V):
         raise ValueError(f"k must be between 0 and {min(MAX_TOP, V)}, got {k}")
-    logprob = torch.empty(n, dtype=torch.float32, device=dev)
-    entropy = torch.empty(n, dtype=torch.float32, device=dev)
-    stat = torch.empty((n, 2), dtype=torch.float32, device=dev)
+    stat = torch.empty((2, n), dtype=torch.float32, device=dev)
+    logprob, entropy = torch.empty((2, n), dtype=torch.float32, device=dev).unbind(0)
     top = None
     if k:
         top = CSR(n, V, torch.empty(n + 1, dtype=torch.int64, device=dev),
@@ -132,8 +131,8 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: Token
     R.same_device(dev, tokens=tokens, g_logprob=g_logprob, g_entropy=g_entropy, stats=stats.stat)
     if tokens.dim() != 1 or tokens.shape[0] != n:
         raise ValueError(f"tokens must be [{n}], got {tuple(tokens.shape)}")
-    if stats.stat.shape[0] != n:
-        raise ValueError(f"stats are of {stats.stat.shape[0]} rows, the logits have {n}")
+    if stats.stat.shape[1] != n:
+        raise ValueError(f"stats are of {stats.stat.shape[1]} rows, the logits have {n}")
     tok = R.token_ids(tokens)
     g, h = R.per_row(g_logprob, n, "g_logprob"), R.per_row(g_entropy, n, "g_entropy")
     inv_t = R.inverse_temperature(stats.temperature)

@@ -151,7 +151,7 @@ def test_grad(dev, dtype, to, accumulate, V, D, n):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["uniform", "zipf", "one token", "all padding", "sorted", "two runs"])
-@pytest.mark.parametrize("n", [2047, 8192, 8193, 20000, 70001])
+@pytest.mark.parametrize("n", [2047, 12288, 12289, 20000, 70001, 140000])
 def test_grad_distributions(kind, n):
     """Both sorts, runs through many tiles, a whole batch of one token."""
     g = gen(n)
