@@ -77,7 +77,10 @@ int lookup(const T* W, int64_t ldw, int64_t V, int64_t D, const void* tok, int w
 
 // ---- sort of (token, position) ------------------------------------------------
 // Keys: the token, or V for padding and for tokens outside the table (sorted
-// last, summed nowhere).
+// last, summed nowhere).  The last pass also writes slot[token], one of the
+// token's places among the sorted keys: a row v has a token if slot[v] is a
+// place and the key there is v, whatever slot[v] held before, so that nothing
+// has to be cleared.
 __device__ __forceinline__ uint32_t key_of(const void* tok, int wide, int64_t i, int64_t V) {
   const int64_t t = token_at(tok, wide, i);
   return (uint32_t)(t >= 0 && t < V ? t : V);
@@ -93,7 +96,8 @@ constexpr int kRankWaves = 16;
 
 __global__ __launch_bounds__(64 * kRankWaves) void embed_rank_sort(const void* __restrict__ tok, int wide, int n,
                                                                    int64_t V, uint32_t* __restrict__ skey,
-                                                                   int32_t* __restrict__ spos) {
+                                                                   int32_t* __restrict__ spos,
+                                                                   int32_t* __restrict__ slot) {
   __shared__ __attribute__((aligned(16))) uint32_t keys[kRankTile];
   __shared__ int part[kRankWaves][64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -138,6 +142,7 @@ __global__ __launch_bounds__(64 * kRankWaves) void embed_rank_sort(const void* _
     for (int q = 0; q < kRankWaves; ++q) at += part[q][lane];
     skey[at] = mine;
     spos[at] = i;
+    if (slot && mine < (uint32_t)V) slot[mine] = at;
   }
 }
 
@@ -262,7 +267,7 @@ __global__ __launch_bounds__(256) void embed_digit_scatter(const void* __restric
                                                            const int32_t* __restrict__ pin, int64_t n, int64_t V,
                                                            int shift, int bits, int64_t tiles, int scanned,
                                                            const int32_t* __restrict__ cnt, uint32_t* __restrict__ kout,
-                                                           int32_t* __restrict__ pout) {
+                                                           int32_t* __restrict__ pout, int32_t* __restrict__ slot) {
   __shared__ int wcnt[4][1 << kMaxBits];
   __shared__ int start[1 << kMaxBits];
   __shared__ int wsum[4];
@@ -314,17 +319,19 @@ __global__ __launch_bounds__(256) void embed_digit_scatter(const void* __restric
     for (int q = 0; q < w; ++q) at += wcnt[q][d];
     kout[at] = k[r];
     pout[at] = pos[r];
+    if (slot && k[r] < (uint32_t)V) slot[k[r]] = at;
   }
 }
 
 // ---- sums ---------------------------------------------------------------------
-// tile: sorted entries a wave of embed_grad_sum
+// tile: sorted entries a wave of embed_grad_sum; fill: table rows a workgroup looks through for
+// empty ones, 0: parts of long rows; fills: such workgroups
 struct GradArgs {
   const void* dy;
   int64_t lddy;
   const uint32_t* skey;
-  const int32_t* spos;
-  int64_t n, V, D, ldw, tile, tiles, slices, vblocks;
+  const int32_t *spos, *slot;
+  int64_t n, V, D, ldw, tile, tiles, slices, fill, fills;
   float scale;
   void* dw;
   float* part;   // [tiles][2][D]: a tile's sums of the run it begins inside and of the one it ends inside
@@ -334,8 +341,8 @@ struct GradArgs {
 // Sorted entries a wave sums: 8 in a short batch, which has few waves to hide
 // their loads behind; 32 else, which writes a quarter of the partial rows.
 constexpr int64_t kShortBatch = 2048;
-constexpr int kFlight = 8;      // row loads in flight
-constexpr int kFillRows = 32;   // table rows a zero-filling wave
+constexpr int kFlight = 8;   // row loads in flight
+constexpr int kFillBytes = 16384, kFillPieces = 8;
 
 // The first of the sorted keys at or behind lo that is not before v: 64 probes a step.
 __device__ __forceinline__ int64_t first_not_before(const uint32_t* __restrict__ skey, int64_t lo, int64_t n, int64_t v) {
@@ -394,33 +401,65 @@ __device__ __forceinline__ void finish_row(const GradArgs& a, int64_t v, int64_t
   store_cols<TO, N>(row, c, from, acc);
 }
 
+__device__ __forceinline__ bool row_is_empty(const GradArgs& a, int64_t v) {
+  const uint32_t at = (uint32_t)a.slot[v];
+  return !((int64_t)at < a.n && (int64_t)a.skey[at] == v);
+}
+
+// Zero rows for tokens that the batch does not have, as pieces of 4 KB of a
+// long row or as groups of short rows.  Eight consecutive workgroups write
+// every eighth piece of their span each, so that the writes in flight lie close
+// together: 1 GiB of such writes takes 166 us, of 32 or 64 KB a workgroup in
+// one stretch 189 and 197.  One piece a workgroup (157) would look for its row
+// each time, which costs more than it gives (470 us).
+template <typename TO>
+__device__ __forceinline__ void fill_piece(const GradArgs& a, int64_t piece) {
+  constexpr int NO = Elem<TO>::kN;
+  const int lane = threadIdx.x & 63;
+  const unsigned nv = (unsigned)(a.D / NO), tail = (unsigned)(a.D % NO);
+  if (a.fill == 0) {
+    const int64_t per = (nv + 255) / 256, pieces = a.V * per;
+    const int64_t base = (piece / 8) * 8 * kFillPieces + piece % 8;
+    if (base >= pieces) return;
+    const int64_t mine = base + 8 * lane;   // lane j looks for the row of piece j
+    const unsigned long long empty = __ballot(lane < kFillPieces && mine < pieces && row_is_empty(a, mine / per));
+#pragma unroll
+    for (int j = 0; j < kFillPieces; ++j) {
+      if (!((empty >> j) & 1)) continue;
+      const int64_t p = base + 8 * j, r = p / per;
+      const unsigned i = (unsigned)(p - r * per) * 256 + threadIdx.x;
+      TO* row = static_cast<TO*>(a.dw) + r * a.ldw;
+      if (i < nv) store_vec(row + (int64_t)i * NO, u32x4{0u, 0u, 0u, 0u});
+      if (p - r * per == per - 1 && threadIdx.x < tail) row[(int64_t)nv * NO + threadIdx.x] = Elem<TO>::cast(0.f);
+    }
+    return;
+  }
+  const int64_t v0 = piece * a.fill;
+  const int rows = (int)(a.V - v0 < a.fill ? a.V - v0 : a.fill);
+  const unsigned long long empty = __ballot(lane < rows && row_is_empty(a, v0 + lane));
+  TO* first = static_cast<TO*>(a.dw) + v0 * a.ldw;
+  for (unsigned i = threadIdx.x; i < rows * nv; i += 256) {
+    const unsigned r = i / nv;
+    if ((empty >> r) & 1) store_vec(first + (int64_t)r * a.ldw + (int64_t)(i - r * nv) * NO, u32x4{0u, 0u, 0u, 0u});
+  }
+  for (unsigned i = threadIdx.x; i < rows * tail; i += 256) {
+    const unsigned r = i / tail;
+    if ((empty >> r) & 1) first[(int64_t)r * a.ldw + (int64_t)nv * NO + (i - r * tail)] = Elem<TO>::cast(0.f);
+  }
+}
+
 template <typename TI, typename TO>
 __global__ __launch_bounds__(256) void embed_grad_sum(GradArgs a) {
   constexpr int N = Elem<TI>::kN;
   const int lane = threadIdx.x & 63;
-  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), waves = (int64_t)gridDim.x * 4;
-  const int64_t sums = a.tiles * a.slices, tasks = sums + a.vblocks;
-  for (int64_t t = wave; t < tasks; t += waves) {
-    if (t >= sums) {   // zero rows for tokens that the batch does not have
-      const int64_t v0 = (t - sums) * kFillRows;
-      int64_t lo = first_not_before(a.skey, 0, a.n, v0), hi = first_not_before(a.skey, lo, a.n, v0 + kFillRows);
-      const int64_t v = v0 + lane, end = hi;   // lane r finds its row between them
-      while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if ((int64_t)a.skey[mid] < v) lo = mid + 1; else hi = mid;
-      }
-      const bool empty = lane < kFillRows && v < a.V && (lo >= end || (int64_t)a.skey[lo] != v);
-      const unsigned long long m = __ballot(empty);
-      constexpr int NO = Elem<TO>::kN;
-      const int64_t nv = a.D / NO;
-      for (int r = 0; r < kFillRows; ++r) {
-        if (!((m >> r) & 1)) continue;
-        TO* row = static_cast<TO*>(a.dw) + (v0 + r) * a.ldw;
-        for (int64_t i = lane; i < nv; i += 64) store_vec(row + i * NO, u32x4{0u, 0u, 0u, 0u});
-        if (nv * NO + lane < a.D) row[nv * NO + lane] = Elem<TO>::cast(0.f);
-      }
+  const int64_t sums = a.tiles * a.slices, sum_groups = (sums + 3) / 4;
+  for (int64_t group = blockIdx.x; group < sum_groups + a.fills; group += gridDim.x) {
+    if (group >= sum_groups) {
+      fill_piece<TO>(a, group - sum_groups);
       continue;
     }
+    const int64_t t = group * 4 + (threadIdx.x >> 6);
+    if (t >= sums) continue;
     const int64_t tile = t / a.slices, c = ((t - tile * a.slices) * 64 + lane) * N;
     const int64_t b = tile * a.tile, e = b + a.tile < a.n ? b + a.tile : a.n;
     const bool mine = c < a.D;
@@ -566,12 +605,12 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_grad_join(GradArgs a) {
 }
 
 struct GradSizes {
-  int64_t tile, tiles, sort_tiles, keys, cnt, total;
+  int64_t tile, tiles, sort_tiles, keys, cnt, slots, total;
   int bits, passes, rounds;
 };
 
-// Layout of the workspace: sorted keys and positions (twice for the radix
-// passes), digit counters, partial rows.
+// Layout of the workspace: sorted keys and positions, slots, the same two again
+// and digit counters for the radix passes, partial rows.
 bool grad_sizes(int64_t n, int64_t V, int64_t D, GradSizes& g) {
   if (n < 0 || n >= (1ll << 31) - (1 << 20) || V < 1 || V >= (1ll << 31) - 1 || D < 1) return false;
   int total_bits = 1;
@@ -585,7 +624,8 @@ bool grad_sizes(int64_t n, int64_t V, int64_t D, GradSizes& g) {
   g.keys = (n + 63) / 64 * 64;
   g.cnt = n > kRankMax ? (g.sort_tiles << g.bits) : 0;
   const int64_t copies = n > kRankMax ? 2 : 1;
-  g.total = (g.keys * 2 * copies + (g.cnt + 63) / 64 * 64 + g.tiles * 2 * D) * 4;
+  g.slots = (V + 63) / 64 * 64;
+  g.total = (g.keys * 2 * copies + g.slots + (g.cnt + 63) / 64 * 64 + g.tiles * 2 * D) * 4;
   return true;
 }
 
@@ -596,9 +636,13 @@ int grad(GradArgs a, hipStream_t s) {
     SPMM_LAUNCH_CHECK();
     return 0;
   }
-  const int64_t waves = a.tiles * a.slices + a.vblocks;
-  if (waves > 0)
-    hipLaunchKernelGGL((embed_grad_sum<TI, TO>), dim3(groups_of((waves + 3) / 4)), dim3(256), 0, s, a);
+  const int64_t row_bytes = a.D * (int64_t)sizeof(TO), groups = (a.tiles * a.slices + 3) / 4;
+  const int64_t pieces = a.V * ((a.D / Elem<TO>::kN + 255) / 256);
+  a.fill = row_bytes >= 2048 ? 0 : row_bytes * 64 <= kFillBytes ? 64 : kFillBytes / row_bytes;
+  a.fills = a.fill ? (a.V + a.fill - 1) / a.fill : (pieces + 8 * kFillPieces - 1) / (8 * kFillPieces) * 8;
+  if (a.accumulate) a.fills = 0;
+  if (groups + a.fills > 0)
+    hipLaunchKernelGGL((embed_grad_sum<TI, TO>), dim3(groups_of(groups + a.fills)), dim3(256), 0, s, a);
   SPMM_LAUNCH_CHECK();
   if (a.tiles > 1) {
     const int64_t joins = a.tiles * ((a.D + 64 * Elem<TO>::kN - 1) / (64 * Elem<TO>::kN));
@@ -635,7 +679,8 @@ SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, c
   int32_t* pa = reinterpret_cast<int32_t*>(ka + g.keys);
   uint32_t* skey = ka;
   int32_t* spos = pa;
-  char* behind = reinterpret_cast<char*>(pa + g.keys);
+  int32_t* slot = accumulate ? nullptr : pa + g.keys;
+  char* behind = reinterpret_cast<char*>(pa + g.keys + g.slots);
   if (n > kRankMax) {
     uint32_t* kb = reinterpret_cast<uint32_t*>(behind);
     int32_t* pb = reinterpret_cast<int32_t*>(kb + g.keys);
@@ -646,17 +691,14 @@ SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, c
     uint32_t* kout = ka;
     int32_t* pout = pa;
     const bool scan = g.sort_tiles > kFewTiles;
+    const dim3 grid((unsigned)g.sort_tiles);
     for (int p = 0; p < g.passes; ++p) {
       const int shift = p * g.bits;
-      const dim3 grid((unsigned)g.sort_tiles);
       hipLaunchKernelGGL(embed_digit_count, grid, dim3(256), 0, s, tok, wide, kin, n, V, shift, g.bits, g.rounds, cnt);
       if (scan) hipLaunchKernelGGL(embed_digit_scan, dim3(1), dim3(1024), 0, s, cnt, g.sort_tiles, g.bits);
-      if (g.rounds == kSmallRounds)
-        hipLaunchKernelGGL((embed_digit_scatter<kSmallRounds>), grid, dim3(256), 0, s, tok, wide, kin, pin, n, V, shift,
-                           g.bits, g.sort_tiles, (int)scan, cnt, kout, pout);
-      else
-        hipLaunchKernelGGL((embed_digit_scatter<kLargeRounds>), grid, dim3(256), 0, s, tok, wide, kin, pin, n, V, shift,
-                           g.bits, g.sort_tiles, (int)scan, cnt, kout, pout);
+      auto scatter = g.rounds == kSmallRounds ? embed_digit_scatter<kSmallRounds> : embed_digit_scatter<kLargeRounds>;
+      hipLaunchKernelGGL(scatter, grid, dim3(256), 0, s, tok, wide, kin, pin, n, V, shift, g.bits, g.sort_tiles,
+                         (int)scan, cnt, kout, pout, p == g.passes - 1 ? slot : nullptr);
       kin = kout;
       pin = pout;
       kout = kout == ka ? kb : ka;
@@ -666,7 +708,7 @@ SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, c
     spos = const_cast<int32_t*>(pin);
   } else if (n > 0) {
     hipLaunchKernelGGL(embed_rank_sort, dim3((unsigned)((n + 63) / 64)), dim3(64 * kRankWaves), 0, s, tok, wide, (int)n,
-                       V, skey, spos);
+                       V, skey, spos, slot);
   }
   SPMM_LAUNCH_CHECK();
   GradArgs a;
@@ -674,13 +716,13 @@ SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, c
   a.lddy = lddy;
   a.skey = skey;
   a.spos = spos;
+  a.slot = slot;
   a.n = n;
   a.V = V;
   a.D = D;
   a.ldw = ldw;
   a.tile = g.tile;
   a.tiles = g.tiles;
-  a.vblocks = accumulate ? 0 : (V + kFillRows - 1) / kFillRows;
   a.scale = scale;
   a.dw = dw;
   a.part = reinterpret_cast<float*>(behind);
