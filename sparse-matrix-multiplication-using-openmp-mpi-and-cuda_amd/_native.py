@@ -88,7 +88,7 @@ def host():
                 _sig(lib, "spmm_cpu_embedding_grad", C.c_int, C.c_int64, C.c_int64, C.c_int64, c_vp, c_vp,
                      C.c_double, c_vp, C.c_int)
                 _sig(lib, "spmm_cpu_token_logprobs", C.c_int, C.c_int64, C.c_int64, c_vp, c_vp, C.c_double, C.c_int,
-                     c_vp, c_vp, c_vp, c_vp, c_vp, C.c_int)
+                     c_vp, c_vp, c_vp, C.c_int)
                 _sig(lib, "spmm_cpu_token_logprobs_grad", C.c_int, C.c_int64, C.c_int64, c_vp, c_vp, C.c_double,
                      c_vp, c_vp, c_vp, c_vp, C.c_int)
                 _sig(lib, "spmm_cpu_distill", C.c_int, C.c_int64, C.c_int64, c_vp, c_vp, c_vp, c_vp, C.c_int64,

@@ -93,9 +93,9 @@ SPMM_HOST_EXPORT int spmm_cpu_embedding_grad(int64_t n, int64_t V, int64_t D, co
   return 0;
 }
 
-// stat: [2][n] maximum, Z.  top_col / top_val: [n][k].
+// stat: [4][n] log-probability, entropy, maximum, Z.  top_col / top_val: [n][k].
 SPMM_HOST_EXPORT int spmm_cpu_token_logprobs(int64_t n, int64_t V, const float* z, const int64_t* tok, double inv_t,
-                                             int k, float* logprob, float* entropy, float* stat, int32_t* top_col,
+                                             int k, float* stat, int32_t* top_col,
                                              float* top_val, int nthreads) {
 #pragma omp parallel num_threads(threads_or_default(nthreads))
   {
@@ -106,10 +106,10 @@ SPMM_HOST_EXPORT int spmm_cpu_token_logprobs(int64_t n, int64_t V, const float* 
       const RowSum r = row_sum(zi, V, inv_t);
       const double o = origin(r.m), logz = r.z == 0 ? 0.0 : std::log(r.z);
       const int64_t t = tok[i];
-      logprob[i] = t >= 0 && t < V ? (float)((zi[t] - o) * inv_t - logz) : (t == -1 ? 0.f : kNan);
-      entropy[i] = r.z == 0 ? 0.f : (float)(logz - r.u / r.z);
-      stat[i] = (float)r.m;
-      stat[n + i] = (float)r.z;
+      stat[i] = t >= 0 && t < V ? (float)((zi[t] - o) * inv_t - logz) : (t == -1 ? 0.f : kNan);
+      stat[n + i] = r.z == 0 ? 0.f : (float)(logz - r.u / r.z);
+      stat[2 * n + i] = (float)r.m;
+      stat[3 * n + i] = (float)r.z;
       if (k > 0) {
         std::iota(idx.begin(), idx.end(), 0);
         std::partial_sort(idx.begin(), idx.begin() + k, idx.end(),
@@ -125,7 +125,7 @@ SPMM_HOST_EXPORT int spmm_cpu_token_logprobs(int64_t n, int64_t V, const float* 
 }
 
 SPMM_HOST_EXPORT int spmm_cpu_token_logprobs_grad(int64_t n, int64_t V, const float* z, const int64_t* tok, double inv_t,
-                                                  const float* entropy, const float* g, const float* h, float* out,
+                                                  const float* stat, const float* g, const float* h, float* out,
                                                   int nthreads) {
 #pragma omp parallel for num_threads(threads_or_default(nthreads))
   for (int64_t i = 0; i < n; ++i) {
@@ -143,14 +143,14 @@ SPMM_HOST_EXPORT int spmm_cpu_token_logprobs_grad(int64_t n, int64_t V, const fl
     const double o = origin(r.m), logz = r.z == 0 ? 0.0 : std::log(r.z);
     for (int64_t j = 0; j < V; ++j) {
       const double lq = (zi[j] - o) * inv_t - logz, q = std::exp(lq);
-      oi[j] = (float)((j == t ? gi : 0.0) - gi * q - (q == 0 ? 0.0 : hi * q * (lq + entropy[i])));
+      oi[j] = (float)((j == t ? gi : 0.0) - gi * q - (q == 0 ? 0.0 : hi * q * (lq + stat[n + i])));
     }
   }
   return 0;
 }
 
-// Teacher entries with column -1 are absent; one outside the vocabulary makes
-// the row's loss and gradient NaN.  out (null: loss only) may be z itself.
+// Teacher entries with column -1 are absent; one outside the vocabulary, or of a
+// value of NaN or +inf, makes the row's loss and gradient NaN.  out (null: loss only) may be z itself.
 SPMM_HOST_EXPORT int spmm_cpu_distill(int64_t n, int64_t V, const float* z, const int64_t* rowptr, const int32_t* col,
                                       const float* val, int64_t nnz, double inv_t, float* loss, float* stat,
                                       const float* weight, float* out, int nthreads) {
@@ -171,6 +171,7 @@ SPMM_HOST_EXPORT int spmm_cpu_distill(int64_t n, int64_t V, const float* z, cons
       const double to = origin(tm);
       for (int64_t k = b; k < e; ++k)
         if (col[k] != -1) ts += std::exp((val[k] - to) * inv_t);
+      bad |= ts != ts;
       const RowSum r = row_sum(zi, V, inv_t);
       const double o = origin(r.m), logz = r.z == 0 ? 0.0 : std::log(r.z);
       double l = 0;

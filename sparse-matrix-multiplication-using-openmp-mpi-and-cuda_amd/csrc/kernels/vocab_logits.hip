@@ -2,9 +2,8 @@
 // entropy and the largest alternatives, distillation from a teacher's stored
 // logits (a CSR matrix), and both gradients.
 //
-// With temperature T and c = log2(e) / T, a row's maximum m and u_j = z_j c - m c
-// (one fma: the product is not rounded, and what rounding m c costs is the same
-// for every j and cancels), e_j = 2^u_j, Z = sum e_j, U = sum e_j u_j:
+// With temperature T, c = log2(e) / T, a row's maximum m, u_j = (z_j - m) c,
+// e_j = 2^u_j, Z = sum e_j, U = sum e_j u_j:
 //   ln q_j  = ln2 (u_j - log2 Z)
 //   entropy = ln2 (log2 Z - U / Z)
 //   dz_j    = [ g (1[j = token] - q_j) - h q_j (ln q_j + entropy) ] / T
@@ -12,10 +11,12 @@
 // A masked place (-inf) has e = 0; a row of nothing else has Z = 0, q = 0.
 //
 // stats    a workgroup holds a segment of one row in registers: one read gives
-//          the maximum, Z, U and the segment's k largest logits.
-// join     a wave (a workgroup with alternatives) puts a row's segments together
-//          and writes the row's results.
-// grad     reads the segment again and writes the gradient.
+//          the maximum, Z, U and, for alternatives, the maxima of groups of
+//          elements.
+// join     a wave puts a row's segments together and writes the row's results.
+//          The k-th largest of the groups' maxima is a lower bound of the k-th
+//          largest logit: only the k groups or so that reach it are read again.
+// grad     reads a segment again and writes its gradient.
 // Long rows of few tokens are split over many workgroups like this, many rows
 // fill the chip the same way; the logits' bytes bound all three.
 #include "vocab_common.hpp"
@@ -25,43 +26,62 @@ using namespace spmm;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kStatsPages = 8, kGradPages = 4;   // pages of 4 KB a workgroup
+constexpr int64_t kFill = 256;   // workgroups, before they get more work each
 constexpr int kMaxTop = 128;     // alternatives a row
-constexpr int kCand = 1024;      // candidates of a segment that are ranked against each other
-constexpr float kHuge = 1e37f;   // row maxima whose product with c may overflow
 constexpr float kLn2 = 0.693147180559945309f;
+
+// ---- a row ----------------------------------------------------------------------
+
+// A row as 16-byte vectors at aligned addresses (unaligned ones cost a quarter
+// of the bandwidth: 820 MB of bf16 rows of odd length 180 us instead of 144),
+// with the elements in front of the first and behind the last one, fewer than
+// a vector each, as up to 2 N - 2 extra elements.
+template <typename T>
+struct Row {
+  static constexpr int N = Elem<T>::kN;
+  const T* z;
+  int V, head, nv;   // columns, elements in front of the first vector, vectors
+  __device__ __forceinline__ Row(const void* base, int64_t ld, int64_t row, int64_t columns) {
+    z = static_cast<const T*>(base) + row * ld;
+    V = (int)columns;
+    head = (int)((0 - reinterpret_cast<uintptr_t>(z)) & 15) / (int)sizeof(T);
+    head = head < V ? head : V;
+    nv = (V - head) / N;
+  }
+  __device__ __forceinline__ u32x4 vec(int v) const {
+    return *reinterpret_cast<const u32x4*>(z + head + (int64_t)v * N);
+  }
+  __device__ __forceinline__ int col(int v) const { return head + v * N; }
+  // column of extra element x of 2 N, or -1
+  __device__ __forceinline__ int extra(int x) const {
+    const int c = x < N ? (x < head ? x : -1) : head + nv * N + (x - N);
+    return x < 2 * N && c < V ? c : -1;
+  }
+};
+
+// How a row's vectors are split over workgroups: pages of 256 vectors (4 KB),
+// VPT of them a workgroup.  Rows of more than VPT pages go to groups of eight
+// workgroups that take every eighth page of their span each: what is in flight
+// at any time then lies close together (1 GiB copied with 32 KB a workgroup:
+// 366 us like this, 402 in one stretch each).  The extra elements belong to the
+// first workgroup.
+struct Walk {
+  int64_t V, S;   // columns, workgroups a row
+  int step;       // 1 or 8
+  __device__ __forceinline__ int page(int seg, int j, int vpt) const {
+    return step == 1 ? seg * vpt + j : ((seg >> 3) * vpt + j) * 8 + (seg & 7);
+  }
+};
+
+// the point that the u_j of a row are measured from
+__device__ __forceinline__ float origin(float m) { return m == -kInf ? 0.f : m; }
+
+__device__ __forceinline__ float exp2_of(float z, float m, float c) { return __builtin_amdgcn_exp2f((z - m) * c); }
+__device__ __forceinline__ float log2_of(float z) { return z == 0.f ? 0.f : __builtin_amdgcn_logf(z); }
 
 struct Part {   // one segment of a row
   float m, z, u, unused;
-};
-
-// u_j of a row whose maximum is m
-template <bool BIG>
-__device__ __forceinline__ float shifted(float z, float m, float mc, float c) {
-  return BIG ? (z - m) * c : __builtin_fmaf(z, c, -mc);
-}
-
-// the row's maximum as the point that the u_j start from; a row of -inf starts from 0
-struct Origin {
-  float m, mc;
-  bool big;
-  __device__ __forceinline__ Origin(float mx, float c) {
-#pragma clang fp contract(off)   // m c is rounded, the same everywhere: no use of it may be fused with the product
-    m = mx == -kInf ? 0.f : mx;
-    mc = m * c;
-    big = !(__builtin_fabsf(m) < kHuge);
-  }
-  __device__ __forceinline__ float at(float z, float c) const {
-    return big ? shifted<true>(z, m, mc, c) : shifted<false>(z, m, mc, c);
-  }
-  // ln q of one logit (natural units throughout where z c might overflow)
-  __device__ __forceinline__ float ln_q(float z, float c, float inv_t, float l2z) const {
-    if (big || !(__builtin_fabsf(z) < kHuge)) return (z - m) * inv_t - kLn2 * l2z;
-    return kLn2 * (shifted<false>(z, m, mc, c) - l2z);
-  }
-  // how far another origin lies from this one, in the same units
-  __device__ __forceinline__ float from(const Origin& o, float c) const {
-    return (big || o.big) ? (o.m - m) * c : o.mc - mc;
-  }
 };
 
 // (value, column) as one number: larger values first, then lower columns; -0 equals +0, NaN is above all
@@ -79,190 +99,71 @@ __device__ __forceinline__ uint64_t entry_of(uint32_t key, int col) {
 }
 __device__ __forceinline__ int col_of(uint64_t entry) { return 0x7fffffff - (int)(uint32_t)entry; }
 
-// Sum of one int per thread over the workgroup (all threads get it); scratch: 4 ints.
-__device__ __forceinline__ int block_sum(int x, int* scratch) {
-  x = wave_sum_i(x);
-  __syncthreads();   // earlier reads of scratch are done
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = x;
-  __syncthreads();
-  return scratch[0] + scratch[1] + scratch[2] + scratch[3];
-}
-
-struct TopLds {
-  uint64_t cand[kCand];
-  float group[kThreads];
-  float bound;
-  int count;
-  int sums[4];
-};
-
-// The k largest of the segment's elements, in order, to list[0 .. k).  Each
-// thread holds r[VPT] vectors (vector j: columns (v0 + j * 256 + tid) * N ..)
-// and one element of the row's tail.  `mine`: the thread's maximum, `odd`:
-// whether it holds a NaN.
-//
-// A k-th largest of the maxima of disjoint groups of elements is a lower bound
-// of the k-th largest element, and few elements reach it: those are ranked
-// against each other.  Where more than kCand do (equal values, masks) the k-th
-// largest key is found bit by bit, and the lowest columns among its equals;
-// that reads the segment again, from the caches, and so costs no registers.
-template <typename T, int VPT>
-__device__ void segment_top(const T* __restrict__ row, const u32x4 (&r)[VPT], int64_t v0, int64_t nv, float tail,
-                            int64_t tail_col, bool has_tail, float mine, bool odd, int64_t held, int k,
-                            uint64_t* __restrict__ list, TopLds& s) {
-  constexpr int N = Elem<T>::kN;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int want = held < k ? (int)held : k;
-  for (int i = want + tid; i < k; i += kThreads) list[i] = 0;   // below every entry
-  if (want == 0) return;   // (uniform: the segment is empty)
-  __syncthreads();
-  s.group[tid] = mine;
-  if (tid == 0) {
-    s.count = 0;
-    s.bound = -kInf;
-  }
-  __syncthreads();
-  if (want <= 64) {   // 64 groups: lane l of all four waves
-    if (w == 0) {
-      const float g = fmaxf(fmaxf(s.group[lane], s.group[64 + lane]), fmaxf(s.group[128 + lane], s.group[192 + lane]));
-      int above = 0;
-#pragma unroll 8
-      for (int j = 0; j < 64; ++j) {
-        const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(g), j));
-        above += (o > g || (o == g && j < lane)) ? 1 : 0;
-      }
-      if (above == want - 1) s.bound = g;
-    }
-  } else if (want <= kThreads) {
-    int above = 0;
-    for (int j = 0; j < kThreads; ++j) {
-      const float o = s.group[j];
-      above += (o > mine || (o == mine && j < tid)) ? 1 : 0;
-    }
-    if (above == want - 1) s.bound = mine;
-  }
-  __syncthreads();
-  const float bound = s.bound;
-  auto push = [&](uint32_t key, int col) {
-    const int at = atomicAdd(&s.count, 1);
-    if (at < kCand) s.cand[at] = entry_of(key, col);
-  };
-  if (mine >= bound || odd) {
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int64_t v = v0 + j * kThreads + tid;
-      if (v >= nv) break;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float z = Elem<T>::get(r[j], i);
-        if (!(z < bound)) push(key_of(z), (int)(v * N + i));
-      }
-    }
-    if (has_tail && !(tail < bound)) push(key_of(tail), (int)tail_col);
-  }
-  __syncthreads();
-  int total = s.count;
-  if (total > kCand) {   // (uniform)
-    auto each = [&](auto&& f) {   // this thread's elements again
-#pragma unroll 1
-      for (int j = 0; j < VPT; ++j) {
-        const int64_t v = v0 + j * kThreads + tid;
-        if (v >= nv) break;
-        const u32x4 x = load_vec(row + v * N);
-#pragma unroll
-        for (int i = 0; i < N; ++i) f(Elem<T>::get(x, i), (int)(v * N + i));
-      }
-      if (has_tail) f(tail, (int)tail_col);
-    };
-    uint32_t key = 0;    // the want-th largest key
-    for (int b = 31; b >= 0; --b) {
-      const uint32_t trial = key | (1u << b);
-      int c = 0;
-      each([&](float z, int) { c += key_of(z) >= trial ? 1 : 0; });
-      if (block_sum(c, s.sums) >= want) key = trial;
-    }
-    int c = 0;
-    each([&](float z, int) { c += key_of(z) > key ? 1 : 0; });
-    const int need = want - block_sum(c, s.sums);   // at least one of the equal ones
-    int below = 0;                                  // the most columns that hold fewer than `need` of them
-    for (int b = 30; b >= 0; --b) {
-      const int trial = below | (1 << b);
-      c = 0;
-      each([&](float z, int col) { c += (key_of(z) == key && col < trial) ? 1 : 0; });
-      if (block_sum(c, s.sums) < need) below = trial;
-    }
-    if (tid == 0) s.count = 0;
-    __syncthreads();
-    each([&](float z, int col) {
-      const uint32_t kz = key_of(z);
-      if (kz > key || (kz == key && col <= below)) push(kz, col);
-    });
-    __syncthreads();
-    total = s.count;
-  }
-  for (int i = tid; i < total; i += kThreads) {
-    const uint64_t e = s.cand[i];
-    int above = 0;
-    for (int j = 0; j < total; ++j) above += s.cand[j] > e ? 1 : 0;
-    if (above < want) list[above] = e;
-  }
-}
+// ---- statistics -------------------------------------------------------------------
 
 struct StatsArgs {
   const void* z;
-  int64_t ld, n, V, S;
+  int64_t ld, n;
+  Walk wk;
   float c;
   Part* part;
-  int k;
-  uint64_t* lists;   // [n * S][k], descending
+  uint32_t* keys;   // [n * S][256 / lanes] the groups' maxima
+  int lanes;        // a group: 1, 2, 4, 8, 16 or 64 neighbouring threads of a workgroup
 };
 
-template <typename T, int EPT, bool ENT, bool TOP>
-__global__ __launch_bounds__(kThreads) void vocab_stats(StatsArgs a) {
-  constexpr int N = Elem<T>::kN, VPT = EPT / N;
-  __shared__ float red[12];
-  __shared__ std::conditional_t<TOP, TopLds, int> top;
+// The statistics of segment t % S of row t / S, by one workgroup.
+template <typename T, int VPT, bool ENT, bool TOP>
+__device__ __forceinline__ void segment_stats(const StatsArgs& a, int64_t t, float* red) {
+  constexpr int N = Elem<T>::kN;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int64_t nv = a.V / N, tasks = a.n * a.S;
-  for (int64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
-    const int64_t row = t / a.S, seg = t - row * a.S;
-    const T* z = static_cast<const T*>(a.z) + row * a.ld;
-    const int64_t v0 = seg * kThreads * VPT;
+  const Walk wk = a.wk;
+  {
+    const int64_t row = t / wk.S;
+    const int seg = (int)(t - row * wk.S);
+    const Row<T> z(a.z, a.ld, row, wk.V);
     u32x4 r[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const int64_t v = v0 + j * kThreads + tid;
+      const int first = wk.page(seg, j, VPT) * kThreads;
+      if (first >= z.nv) break;   // (uniform)
       r[j] = u32x4{Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf};
-      if (v < nv) r[j] = load_vec(z + v * N);
+      if (first + tid < z.nv) r[j] = z.vec(first + tid);
     }
-    const int64_t tail_col = nv * N + tid;
-    const bool has_tail = seg == a.S - 1 && tail_col < a.V;
-    const float tail = has_tail ? Elem<T>::load(z + tail_col) : -kInf;
-    float mx = tail;
+    const int extra = seg == 0 ? z.extra(tid) : -1;
+    const float tail = extra >= 0 ? Elem<T>::load(z.z + extra) : -kInf;
+    typename Elem<T>::Max most;
+    most.one(tail);
 #pragma unroll
-    for (int j = 0; j < VPT; ++j)
-#pragma unroll
-      for (int i = 0; i < N; ++i) mx = fmaxf(mx, Elem<T>::get(r[j], i));
-    const float wm = wave_max(mx);
+    for (int j = 0; j < VPT; ++j) {
+      if (wk.page(seg, j, VPT) * kThreads >= z.nv) break;
+      most.vec(r[j]);
+    }
+    const float mx = most.get(), wm = wave_max(mx);
     if (lane == 0) red[w] = wm;
     __syncthreads();
-    const float m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const Origin o(m, a.c);
+    const float m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), o = origin(m);
     float zs = 0.f, us = 0.f;
-    auto sum = [&](auto big) {
-      auto add = [&](float z) {
-        const float u = shifted<decltype(big)::value>(z, o.m, o.mc, a.c);
-        const float e = __builtin_amdgcn_exp2f(u);
+    auto sum = [&](auto masked) {
+      zs = us = 0.f;
+      auto add = [&](float x) {
+        const float u = (x - o) * a.c, e = __builtin_amdgcn_exp2f(u);
         zs += e;
-        if (ENT) us = __builtin_fmaf(e, fmaxf(u, -1e30f), us);   // (0 times -inf)
+        if (ENT) us = __builtin_fmaf(e, decltype(masked)::value ? fmaxf(u, -1e30f) : u, us);
       };
-      add(tail);
+      if (extra >= 0) add(tail);
 #pragma unroll
-      for (int j = 0; j < VPT; ++j)
+      for (int j = 0; j < VPT; ++j) {
+        const int first = wk.page(seg, j, VPT) * kThreads;
+        if (first >= z.nv) break;
+        if (first + tid < z.nv) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) add(Elem<T>::get(r[j], i));
+          for (int i = 0; i < N; ++i) add(Elem<T>::get(r[j], i));
+        }
+      }
     };
-    if (o.big) sum(std::true_type()); else sum(std::false_type());
+    sum(std::false_type());
+    // 0 times -inf spoils U where places are masked: only such waves keep u finite (one instruction an element)
+    if (ENT && __ballot(us != us)) sum(std::true_type());
     const float zw = wave_sum(zs), uw = ENT ? wave_sum(us) : 0.f;
     if (lane == 0) {
       red[4 + w] = zw;
@@ -272,13 +173,27 @@ __global__ __launch_bounds__(kThreads) void vocab_stats(StatsArgs a) {
     if (tid == 0)
       a.part[t] = Part{m, (red[4] + red[5]) + (red[6] + red[7]), (red[8] + red[9]) + (red[10] + red[11]), 0.f};
     if constexpr (TOP) {
-      const int64_t left = (nv - v0) * N + (seg == a.S - 1 ? a.V - nv * N : 0);
-      const int64_t whole = (int64_t)kThreads * EPT + (seg == a.S - 1 ? a.V - nv * N : 0);
-      segment_top<T, VPT>(z, r, v0, nv, tail, tail_col, has_tail, mx, zs != zs, left < whole ? left : whole, a.k,
-                          a.lists + t * a.k, top);
+      uint32_t key = key_of(mx);
+      if (!(zs < kInf)) {   // a NaN among this thread's elements, or +inf
+        key = key_of(tail);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+          if (wk.page(seg, j, VPT) * kThreads >= z.nv) break;
+#pragma unroll
+          for (int i = 0; i < N; ++i) key = max_u(key, key_of(Elem<T>::get(r[j], i)));
+        }
+      }
+      key = a.lanes == 64 ? over_wave(key, max_u) : over_lanes(key, a.lanes, max_u);
+      if ((tid & (a.lanes - 1)) == 0) a.keys[t * (kThreads / a.lanes) + tid / a.lanes] = key;
     }
     __syncthreads();   // red is written again
   }
+}
+
+template <typename T, int VPT, bool TOP>
+__global__ __launch_bounds__(kThreads) void vocab_stats(StatsArgs a) {
+  __shared__ float red[12];
+  for (int64_t t = blockIdx.x; t < a.n * a.wk.S; t += gridDim.x) segment_stats<T, VPT, true, TOP>(a, t, red);
 }
 
 // A row's segments put together by one wave (all lanes get the result).
@@ -290,169 +205,372 @@ __device__ __forceinline__ RowStat join_parts(const Part* p, int64_t S, float c)
   float m = -kInf;
   for (int64_t s = lane; s < S; s += 64) m = fmaxf(m, p[s].m);
   m = wave_max(m);
-  const Origin o(m, c);
+  const float o = origin(m);
   float z = 0.f, u = 0.f;
   for (int64_t s = lane; s < S; s += 64) {
     const Part q = p[s];
-    const float d = o.from(Origin(q.m, c), c), f = q.m == -kInf ? 1.f : __builtin_amdgcn_exp2f(d);
-    // a segment of -inf alone has z = 0, unless it holds a NaN
+    // (a segment of -inf alone has z = 0 unless it holds a NaN)
+    const float d = (origin(q.m) - o) * c, f = q.m == -kInf ? 1.f : __builtin_amdgcn_exp2f(d);
     z += q.z * f;
-    u += f == 0.f ? 0.f : f * (q.u + q.z * (q.m == -kInf ? 0.f : d));
+    u += f == 0.f ? 0.f : f * (q.u + (q.m == -kInf ? 0.f : q.z * d));
   }
-  return RowStat{m, wave_sum(z), wave_sum(u)};
+  z = wave_sum(z);
+  return RowStat{m, z < kInf ? z : __builtin_nanf(""), wave_sum(u)};   // (+inf among the logits)
 }
+
+// ---- log-probabilities ------------------------------------------------------------
 
 struct JoinArgs {
   const void* z;
-  int64_t ld, n, V, S;
+  int64_t ld, n;
+  Walk wk;
+  int vpt;
   float c, inv_t;
   const Part* part;
   const void* tok;
-  int wide, k;
-  const uint64_t* lists;
-  float *logprob, *entropy, *stat;   // stat: [2][n] maximum and Z
+  int wide, k, lanes;
+  const uint32_t* keys;
+  float* stat;   // [4][n] log-probability, entropy, maximum, Z
   int64_t* rowptr;
   int32_t* top_col;
   float* top_val;
 };
 
-constexpr int kMergeLds = 2048;   // entries of a row's lists that are merged in LDS
+constexpr int kCand = 512;      // candidates of a row that are ranked against each other
+constexpr int kHits = 256;      // groups of a row that are read again
+constexpr int kKeyRegs = 16;    // groups of a row whose maxima a lane keeps
+constexpr int kFlight = 2;      // vectors of a lane that are read at a time (8: 13 KB of LDS a wave, half the waves)
 
+struct TopLds {   // of one wave
+  u32x4 vec[kFlight][64];
+  uint64_t cand[kCand + 8];
+  int hit[kHits];
+};
+
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// sum of x over the lanes up to and with this one
+__device__ __forceinline__ int wave_scan(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+// The k largest logits of a row, in order, to out[0 .. k), by one wave.
+//
+// `from`, a key that at least k elements reach, starts as the k-th largest of
+// the groups' maxima.  The elements that reach it are collected from the groups
+// whose maxima do.  More than kCand: the k-th largest of those in hand is a
+// better bound, or, if it is the same one, only elements above it are
+// collected, and of its equals the lowest columns are looked up in the row.
+//
+// A wave runs this once, alone on its SIMD or nearly so, and its time goes into
+// round trips to memory and into fetching code that no wave has run before: the
+// loops are kept short and not unrolled.
+template <typename T, typename F>
+__device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& s, F&& out) {
+  constexpr int N = Elem<T>::kN;
+  const int lane = threadIdx.x & 63, k = a.k;
+  const unsigned long long below = (1ull << lane) - 1ull;
+  const Row<T> z(a.z, a.ld, row, a.wk.V);
+  // vectors a group, and what else is a power of two, as shifts
+  const int lanes_log = __builtin_ctz(a.lanes), slots_log = lanes_log + __builtin_ctz(a.vpt), per_log = 8 - lanes_log;
+  const int groups = (int)(a.wk.S << per_log);
+  const uint32_t* keys = a.keys + row * groups;
+  const bool in_regs = groups <= 64 * kKeyRegs;
+  uint32_t held[kKeyRegs];
+#pragma unroll
+  for (int j = 0; j < kKeyRegs; ++j) held[j] = in_regs && j * 64 + lane < groups ? keys[j * 64 + lane] : 0u;
+  // f(i, key) for all lanes' groups (a lane behind the last has key 0)
+  auto each_key = [&](auto&& f) {
+    if (in_regs) {
+#pragma unroll
+      for (int j = 0; j < kKeyRegs; ++j) {
+        if (j * 64 >= groups) break;
+        f(j * 64 + lane, held[j]);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < groups; i += 64) f(i + lane, i + lane < groups ? keys[i + lane] : 0u);
+    }
+  };
+
+  // the k-th largest key, bit by bit; reach(key): how many are not below it
+  auto kth_largest = [&](auto&& reach) {
+    uint32_t key = 0;
+#pragma unroll 1
+    for (int b = 31; b >= Elem<T>::kLowBits; --b) {
+      const uint32_t trial = key | (1u << b);
+      if (reach(trial) >= k) key = trial;
+    }
+    // the bits that the type does not have: ones in negative keys and in NaN's
+    if (!(key & 0x80000000u) || key > key_of(kInf)) key |= (1u << Elem<T>::kLowBits) - 1u;
+    return key;
+  };
+  // (64 bits: it may pass the largest key)
+  uint64_t from = kth_largest([&](uint32_t trial) {
+    int c = 0;
+    each_key([&](int, uint32_t key) { c += __popcll(__ballot(key >= trial)); });
+    return c;
+  });
+  bool equals = false;   // whether elements of key from - 1 belong to the k largest too
+  if (from == key_of(-kInf)) {   // fewer than k groups hold anything else
+    ++from;
+    equals = true;
+  }
+  int count;
+#pragma unroll 1
+  for (;;) {
+    int hits = 0;
+#pragma unroll 1
+    for (;;) {
+      hits = 0;
+      each_key([&](int i, uint32_t key) {
+        const unsigned long long m = __ballot(key >= from);
+        if (m == 0) return;
+        const int at = hits + __popcll(m & below);
+        if (key >= from && at < kHits) s.hit[at] = i;
+        hits += __popcll(m);
+      });
+      if (hits <= kHits) break;
+      ++from;   // more than k equal maxima; fewer than k are above them
+      equals = true;
+    }
+    wave_fence();
+    count = 0;
+    const bool only_nan = from > key_of(kInf);
+    const float bound = only_nan ? 0.f : value_of((uint32_t)from);
+    auto reaches = [&](float x) { return only_nan ? x != x && from <= 0xffffffffu : !(x < bound); };
+    auto offer = [&](bool in, float x, int col) {   // (most lanes have nothing)
+      const unsigned long long m = __ballot(in && reaches(x));
+      if (m == 0) return;
+      const int at = count + __popcll(m & below);
+      if (((m >> lane) & 1) && at < kCand) s.cand[at] = entry_of(key_of(x), col);
+      count += __popcll(m);
+    };
+    const int vecs = hits << slots_log;
+    auto place = [&](int i) {   // vector i of the hits, or -1
+      if (i >= vecs) return -1;
+      const int g = s.hit[i >> slots_log], slot = i & ((1 << slots_log) - 1);
+      const int thread = ((g << lanes_log) & 255) + (slot & (a.lanes - 1));
+      const int v = a.wk.page(g >> per_log, slot >> lanes_log, a.vpt) * kThreads + thread;
+      return v < z.nv ? v : -1;
+    };
+#pragma unroll 1
+    for (int i0 = 0; i0 < vecs; i0 += 64 * kFlight) {
+      u32x4 x[kFlight];
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) {
+        const int v = place(i0 + f * 64 + lane);
+        x[f] = z.vec(v < 0 ? 0 : v);   // (there is a vector, or no group would be hit)
+      }
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) s.vec[f][lane] = x[f];
+      wave_fence();
+#pragma unroll 1
+      for (int f = 0; f < kFlight && i0 + f * 64 < vecs; ++f) {
+        const int v = place(i0 + f * 64 + lane);
+        const u32x4 y = s.vec[f][lane];
+#pragma unroll
+        for (int e = 0; e < N; ++e) offer(v >= 0, Elem<T>::get(y, e), z.col(v) + e);
+      }
+      wave_fence();
+    }
+    {
+      const int c = z.extra(lane);
+      offer(c >= 0, c >= 0 ? Elem<T>::load(z.z + c) : 0.f, c);
+    }
+    wave_fence();
+    if (count <= kCand) break;
+    const uint32_t better = kth_largest([&](uint32_t trial) {
+      int c = 0;
+#pragma unroll 1
+      for (int i = 0; i < kCand; i += 64) c += __popcll(__ballot((uint32_t)(s.cand[i + lane] >> 32) >= trial));
+      return c;
+    });
+    equals = better == from;
+    from = equals ? from + 1 : better;
+  }
+  // of the equals of from - 1 the lowest columns, as many as are missing: the
+  // extra elements in front of the vectors, the vectors in order, those behind
+  if (equals && count < k) {
+    const uint32_t level = (uint32_t)(from - 1);
+    const int rounds = (z.nv + 63) / 64;
+#pragma unroll 1
+    for (int r = -1; r <= rounds && count < k; ++r) {
+      const bool vec = r >= 0 && r < rounds && r * 64 + lane < z.nv;
+      const int first = r < 0 ? lane : r < rounds ? z.col(r * 64 + lane) : z.col(z.nv) + lane;
+      const int elems = vec ? N : (r < 0 ? lane < z.head : r == rounds && first < z.V) ? 1 : 0;
+      int many = 0;
+      for (int e = 0; e < elems; ++e) many += key_of(Elem<T>::load(z.z + first + e)) == level ? 1 : 0;
+      const int incl = wave_scan(many);
+      int at = count + incl - many;
+      for (int e = 0; e < elems && at < k; ++e)
+        if (key_of(Elem<T>::load(z.z + first + e)) == level) s.cand[at++] = entry_of(level, first + e);
+      count += __builtin_amdgcn_readlane(incl, 63);
+    }
+    count = count < k ? count : k;
+    wave_fence();
+  }
+  constexpr int kRead = 8;   // candidates read at a time: the list is filled up with entries below all others
+  if (lane < kRead) s.cand[count + lane] = 0;
+  wave_fence();
+#pragma unroll 1
+  for (int i = lane; i < count; i += 64) {
+    const uint64_t e = s.cand[i];
+    int above = 0;
+#pragma unroll 1
+    for (int j = 0; j < count; j += kRead) {
+      uint64_t o[kRead];
+#pragma unroll
+      for (int u = 0; u < kRead; ++u) o[u] = s.cand[j + u];
+#pragma unroll
+      for (int u = 0; u < kRead; ++u) above += o[u] > e ? 1 : 0;
+    }
+    if (above < k) out(above, e);
+  }
+  wave_fence();
+}
+
+// A wave a row.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void vocab_join(JoinArgs a) {
-  __shared__ uint64_t lds[TOP ? kMergeLds : 1];
+  __shared__ std::conditional_t<TOP, TopLds, int> top[4];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t rows = TOP ? a.n : (a.n + 3) / 4;
-  for (int64_t t = blockIdx.x; t < rows; t += gridDim.x) {
-    const int64_t row = TOP ? t : t * 4 + w;
-    if (row >= a.n) return;   // (only without alternatives: no barrier follows)
-    const RowStat st = join_parts(a.part + row * a.S, a.S, a.c);
-    const Origin o(st.m, a.c);
-    const float l2z = st.z == 0.f ? 0.f : __builtin_amdgcn_logf(st.z);
-    if (lane == 0 && (!TOP || w == 0)) {
-      const int64_t id = token_at(a.tok, a.wide, row);
-      float lp = 0.f;   // padding
-      if (id >= 0 && id < a.V)
-        lp = o.ln_q(Elem<T>::load(static_cast<const T*>(a.z) + row * a.ld + id), a.c, a.inv_t, l2z);
-      else if (id != -1)
-        lp = __builtin_nanf("");
-      a.logprob[row] = lp;
-      a.entropy[row] = st.z == 0.f ? 0.f : kLn2 * (l2z - st.u / st.z);
-      a.stat[row] = st.m;
-      a.stat[a.n + row] = st.z;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + w; row < a.n; row += (int64_t)gridDim.x * 4) {
+    const T* z = static_cast<const T*>(a.z) + row * a.ld;
+    const int64_t id = token_at(a.tok, a.wide, row);
+    const bool inside = id >= 0 && id < a.wk.V;
+    const float x = Elem<T>::load(z + (inside ? id : 0));
+    const RowStat st = join_parts(a.part + row * a.wk.S, a.wk.S, a.c);
+    const float o = origin(st.m), l2z = log2_of(st.z);
+    auto ln_q = [&](float y) { return (y - o) * a.inv_t - kLn2 * l2z; };
+    if (lane == 0) {
+      a.stat[row] = inside ? ln_q(x) : id == -1 ? 0.f : __builtin_nanf("");   // (-1: padding)
+      a.stat[a.n + row] = st.z == 0.f ? 0.f : kLn2 * (l2z - st.u / st.z);
+      a.stat[2 * a.n + row] = st.m;
+      a.stat[3 * a.n + row] = st.z;
     }
     if constexpr (TOP) {
-      // every entry's place: how many of the other segments' (descending) lists are above it
-      const int k = a.k;
-      const int64_t m = a.S * k;
-      const uint64_t* all = a.lists + row * m;
-      const bool in_lds = m <= kMergeLds;
-      __syncthreads();
-      if (in_lds)
-        for (int64_t i = threadIdx.x; i < m; i += kThreads) lds[i] = all[i];
-      __syncthreads();
-      const uint64_t* src = in_lds ? lds : all;
-      for (int64_t i = threadIdx.x; i < m; i += kThreads) {
-        const uint64_t e = src[i];
-        if (e == 0) continue;   // a segment shorter than k
-        const int64_t own = i / k;
-        int place = (int)(i - own * k);
-        for (int64_t s = 0; s < a.S && place < k; ++s) {
-          if (s == own) continue;
-          const uint64_t* l = src + s * k;
-          int lo = 0, hi = k;   // entries above e
-          while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (l[mid] > e) lo = mid + 1; else hi = mid;
-          }
-          place += lo;
-        }
-        if (place < k) {
-          a.top_col[row * k + place] = col_of(e);
-          a.top_val[row * k + place] = o.ln_q(value_of((uint32_t)(e >> 32)), a.c, a.inv_t, l2z);
-        }
+      if (lane == 0) {
+        a.rowptr[row] = row * a.k;
+        if (row == a.n - 1) a.rowptr[a.n] = a.n * a.k;
       }
-      if (threadIdx.x == 0) {
-        a.rowptr[row] = row * k;
-        if (row == a.n - 1) a.rowptr[a.n] = a.n * k;
-      }
+      row_top<T>(a, row, top[w], [&](int place, uint64_t e) {
+        a.top_col[row * a.k + place] = col_of(e);
+        a.top_val[row * a.k + place] = ln_q(value_of((uint32_t)(e >> 32)));
+      });
     }
   }
 }
 
+// ---- gradients --------------------------------------------------------------------
+
+// This thread's places of a segment: read at once, written as f(z) later.  An
+// output whose rows lie at another alignment than the logits' gets unaligned
+// stores.
+template <typename T, int VPT>
+struct Segment {
+  static constexpr int N = Elem<T>::kN;
+  u32x4 r[VPT];
+  float tail;
+  int extra;
+  __device__ __forceinline__ Segment(const Row<T>& z, const Walk& wk, int seg) {
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int v = wk.page(seg, j, VPT) * kThreads + (int)threadIdx.x;
+      if (v < z.nv) r[j] = z.vec(v);
+    }
+    extra = seg == 0 ? z.extra(threadIdx.x) : -1;
+    tail = extra >= 0 ? Elem<T>::load(z.z + extra) : 0.f;
+  }
+  template <typename F>
+  __device__ __forceinline__ void write(const Row<T>& z, T* out, const Walk& wk, int seg, F&& f) const {
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int v = wk.page(seg, j, VPT) * kThreads + (int)threadIdx.x;
+      if (v >= z.nv) break;
+      float x[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = Elem<T>::get(r[j], i);
+      f(x, z.col(v), std::integral_constant<int, N>());
+      store_vec(out + z.col(v), Elem<T>::pack(x));
+    }
+    if (extra >= 0) {
+      float x[1] = {tail};
+      f(x, extra, std::integral_constant<int, 1>());
+      out[extra] = Elem<T>::cast(x[0]);
+    }
+  }
+};
+
+template <typename T, int VPT>
+__device__ __forceinline__ void zero_segment(const Row<T>& z, T* out, const Walk& wk, int seg) {
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int v = wk.page(seg, j, VPT) * kThreads + (int)threadIdx.x;
+    if (v < z.nv) store_vec(out + z.col(v), u32x4{0u, 0u, 0u, 0u});
+  }
+  const int extra = seg == 0 ? z.extra(threadIdx.x) : -1;
+  if (extra >= 0) out[extra] = Elem<T>::cast(0.f);
+}
+
 struct TokenGradArgs {
   const void* z;
-  int64_t ld, n, V, S;
+  int64_t ld, n;
+  Walk wk;
   float c, inv_t;
   const void* tok;
   int wide;
-  const float *stat, *entropy, *g, *h;   // g, h: null = 0
+  const float *stat, *g, *h;   // g, h: null = 0
   void* out;
   int64_t ldo;
 };
 
 // dz_j = e_j (alpha + beta u_j), plus g / T at the token
-template <typename T, int EPT, bool ENT>
+template <typename T, int VPT, bool ENT>
 __global__ __launch_bounds__(kThreads) void vocab_token_grad(TokenGradArgs a) {
-  constexpr int N = Elem<T>::kN, VPT = EPT / N;
-  const int tid = threadIdx.x;
-  const int64_t nv = a.V / N, tasks = a.n * a.S;
+  const Walk wk = a.wk;
+  const int64_t tasks = a.n * wk.S;
   for (int64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
-    const int64_t row = t / a.S, seg = t - row * a.S;
-    const T* z = static_cast<const T*>(a.z) + row * a.ld;
+    const int64_t row = t / wk.S;
+    const int seg = (int)(t - row * wk.S);
+    const Row<T> z(a.z, a.ld, row, wk.V);
     T* out = static_cast<T*>(a.out) + row * a.ldo;
-    const int64_t v0 = seg * kThreads * VPT, tail_col = nv * N + tid;
-    const bool has_tail = seg == a.S - 1 && tail_col < a.V;
-    int64_t id = token_at(a.tok, a.wide, row);
-    float g = a.g ? a.g[row] * a.inv_t : 0.f;
+    const int64_t id = token_at(a.tok, a.wide, row);
+    float g = a.g && id != -1 ? a.g[row] * a.inv_t : 0.f;
     const float h = ENT ? a.h[row] * a.inv_t : 0.f;
-    if (id == -1) g = 0.f;
     if (g == 0.f && h == 0.f) {   // nothing flows into this row: its logits are not read
-      const float zero[N] = {};
-#pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        const int64_t v = v0 + j * kThreads + tid;
-        if (v < nv) store_vec(out + v * N, Elem<T>::pack(zero));
-      }
-      if (has_tail) out[tail_col] = Elem<T>::cast(0.f);
+      zero_segment<T, VPT>(z, out, wk, seg);
       continue;
     }
-    if (id < -1 || id >= a.V) g = __builtin_nanf("");
-    const float Z = a.stat[a.n + row], l2z = Z == 0.f ? 0.f : __builtin_amdgcn_logf(Z), rz = Z == 0.f ? 0.f : 1.f / Z;
-    const Origin o(a.stat[row], a.c);
-    const float beta = -h * kLn2 * rz, alpha = -(g + (ENT ? h * (a.entropy[row] - kLn2 * l2z) : 0.f)) * rz;
-    u32x4 r[VPT];
+    const Segment<T, VPT> part(z, wk, seg);
+    if (id < -1 || id >= wk.V) g = __builtin_nanf("");
+    const float Z = a.stat[3 * a.n + row], l2z = log2_of(Z), rz = Z == 0.f ? 0.f : 1.f / Z;
+    const float o = origin(a.stat[2 * a.n + row]);
+    const float beta = -h * kLn2 * rz, alpha = -(g + (ENT ? h * (a.stat[a.n + row] - kLn2 * l2z) : 0.f)) * rz;
+    part.write(z, out, wk, seg, [&](float* x, int col, auto n) {
+      constexpr int n_ = decltype(n)::value;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int64_t v = v0 + j * kThreads + tid;
-      if (v < nv) r[j] = load_vec(z + v * N);
-    }
-    auto write = [&](auto big) {
-      auto grad = [&](float x) {
-        const float u = shifted<decltype(big)::value>(x, o.m, o.mc, a.c), e = __builtin_amdgcn_exp2f(u);
-        return ENT ? e * __builtin_fmaf(beta, fmaxf(u, -1e30f), alpha) : e * alpha;
-      };
-#pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        const int64_t v = v0 + j * kThreads + tid;
-        if (v >= nv) break;
-        float x[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = grad(Elem<T>::get(r[j], i));
-        const int64_t at = id - v * N;
-        if (at >= 0 && at < N) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) x[i] += i == (int)at ? g : 0.f;
-        }
-        store_vec(out + v * N, Elem<T>::pack(x));
+      for (int i = 0; i < n_; ++i) {
+        const float u = (x[i] - o) * a.c, e = __builtin_amdgcn_exp2f(u);
+        x[i] = ENT ? e * __builtin_fmaf(beta, fmaxf(u, -1e30f), alpha) : e * alpha;   // (0 times -inf)
       }
-      if (has_tail) out[tail_col] = Elem<T>::cast(grad(Elem<T>::load(z + tail_col)) + (id == tail_col ? g : 0.f));
-    };
-    if (o.big) write(std::true_type()); else write(std::false_type());
+      const int64_t at = id - col;
+      if (at >= 0 && at < n_) {
+#pragma unroll
+        for (int i = 0; i < n_; ++i) x[i] += i == (int)at ? g : 0.f;
+      }
+    });
   }
 }
 
-// ---- distillation -------------------------------------------------------------
+// ---- distillation -------------------------------------------------------------------
+
 struct Teacher {
   const int64_t* rowptr;
   const int32_t* col;
@@ -475,9 +593,11 @@ struct Teacher {
 
 struct DistillArgs {
   const void* z;
-  int64_t ld, n, V, S;
+  int64_t ld, n, V;
+  Walk wk;
   float c, inv_t;
   const Part* part;
+  int64_t S;            // segments a row in part
   Teacher t;
   float *loss, *stat;   // stat: [n][4] maximum, Z, teacher's maximum and sum
   float* picked;        // [nnz] the student's logits at the teacher's entries
@@ -486,9 +606,10 @@ struct DistillArgs {
   int64_t ldo;
 };
 
-// Teacher's statistics and the loss of one row, by one wave.
+// A row of the teacher by one wave: its maximum and sum, and the student's
+// logits at its entries, which an output in place of the logits overwrites.
 template <typename T>
-__device__ __forceinline__ void distill_row(const DistillArgs& a, int64_t row, RowStat st) {
+__device__ __forceinline__ void pick_row(const DistillArgs& a, int64_t row) {
   const int lane = threadIdx.x & 63;
   int64_t b, e;
   a.t.range(row, b, e);
@@ -499,158 +620,183 @@ __device__ __forceinline__ void distill_row(const DistillArgs& a, int64_t row, R
     const int32_t col = a.t.col[i];
     bad |= col < -1 || col >= a.V;
     if (col != -1) tm = fmaxf(tm, a.t.at(i));
+    if (col >= 0 && col < a.V) a.picked[i] = Elem<T>::load(z + col);
   }
-  tm = wave_max(tm);
-  const float tm0 = tm == -kInf ? 0.f : tm;
+  tm = origin(wave_max(tm));
+  bad = __ballot(bad) != 0;
   float ts = 0.f;
   for (int64_t i = b + lane; i < e; i += 64)
-    if (a.t.col[i] != -1) ts += __builtin_amdgcn_exp2f((a.t.at(i) - tm0) * a.c);
+    if (a.t.col[i] != -1) ts += exp2_of(a.t.at(i), tm, a.c);
   ts = wave_sum(ts);
-  const Origin o(st.m, a.c);
-  const float l2z = st.z == 0.f ? 0.f : __builtin_amdgcn_logf(st.z), l2t = __builtin_amdgcn_logf(ts);
-  float loss = 0.f;
-  for (int64_t i = b + lane; i < e; i += 64) {
-    const int32_t col = a.t.col[i];
-    if (col < 0 || col >= a.V) continue;
-    const float x = Elem<T>::load(z + col);
-    a.picked[i] = x;
-    const float u = (a.t.at(i) - tm0) * a.c, p = __builtin_amdgcn_exp2f(u) / ts;
-    if (!(p == 0.f)) loss += p * (kLn2 * (u - l2t) - o.ln_q(x, a.c, a.inv_t, l2z));
-  }
-  loss = wave_sum(loss);
-  if (__ballot(bad)) loss = st.z = __builtin_nanf("");   // a column outside the vocabulary
-  if (ts == 0.f) loss = __ballot(bad) ? loss : 0.f;      // no mass: nothing to learn
   if (lane == 0) {
-    a.loss[row] = loss;
-    a.stat[row * 4] = st.m;
-    a.stat[row * 4 + 1] = st.z;
-    a.stat[row * 4 + 2] = tm0;
-    a.stat[row * 4 + 3] = __ballot(bad) ? __builtin_nanf("") : ts;
+    a.stat[row * 4 + 2] = tm;
+    a.stat[row * 4 + 3] = bad ? __builtin_nanf("") : ts;   // (a column outside the vocabulary)
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_join(DistillArgs a) {
-  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.n; row += (int64_t)gridDim.x * 4)
-    distill_row<T>(a, row, join_parts(a.part + row * a.S, a.S, a.c));
-}
-
-constexpr int kEntries = 1024;   // teacher entries staged in LDS
-
-struct EntryLds {
-  int32_t col[kEntries];
-  float p[kEntries];
-};
-
-// Columns [lo, hi) of a row's gradient where the teacher has entries, written
-// over what the dense pass left there: w (q - p) / T with the p of equal
-// columns summed in their order, rounded once.  All threads of the workgroup;
-// `scale` = w / (T Z), `wt` = w / T.
-template <typename T>
-__device__ __forceinline__ void distill_entries(const DistillArgs& a, int64_t row, int64_t lo, int64_t hi,
-                                                const Origin& o, float scale, float wt, float tm, float ts, T* out,
-                                                EntryLds& s) {
-  int64_t b, e;
-  a.t.range(row, b, e);
-  for (int64_t base = b; base < e; base += blockDim.x) {
-    const int64_t i = base + threadIdx.x;
-    const int32_t mine = i < e ? a.t.col[i] : -1;
-    bool first = mine >= lo && mine < hi;
-    float p = 0.f;
-    for (int64_t from = b; from < e; from += kEntries) {
-      const int count = (int)(e - from < kEntries ? e - from : kEntries);
-      __syncthreads();
-      for (int j = threadIdx.x; j < count; j += blockDim.x) {
-        s.col[j] = a.t.col[from + j];
-        s.p[j] = __builtin_amdgcn_exp2f((a.t.at(from + j) - tm) * a.c) / ts;
-      }
-      __syncthreads();
-      if (first) {
-        for (int j = 0; j < count; ++j) {
-          const bool same = s.col[j] == mine;
-          first = first && !(same && from + j < i);
-          p += same ? s.p[j] : 0.f;
-        }
-      }
+// Statistics of the rows' segments and, in further workgroups, the teacher's.
+template <typename T, int VPT>
+__global__ __launch_bounds__(kThreads) void distill_stats(StatsArgs s, DistillArgs a) {
+  __shared__ float red[12];
+  const int64_t segments = a.n * s.wk.S, groups = segments + (a.n + 3) / 4;
+  for (int64_t t = blockIdx.x; t < groups; t += gridDim.x) {
+    if (t < segments) {
+      segment_stats<T, VPT, false, false>(s, t, red);
+    } else {
+      const int64_t row = (t - segments) * 4 + (threadIdx.x >> 6);
+      if (row < a.n) pick_row<T>(a, row);
     }
-    if (first)
-      out[mine] = Elem<T>::cast(__builtin_amdgcn_exp2f(o.at(a.picked[i], a.c)) * scale - wt * p);
   }
 }
 
-template <typename T, int EPT>
+// w q / T everywhere.  JOIN: the rows' statistics are put together here, from
+// their segments'.
+//
+// Bytes bound a step of loss and gradient: the logits are read twice and the
+// gradient written once, 3.2 GB for 4096 x 131072 bf16 in 580 us (519 at the
+// rate of a large copy).  One read would take a row of 256 KB in registers
+// from its statistics to its gradient, half of a CU's: a workgroup a row with
+// half of it kept took 574 us, with all of it spilling 670.  A second read out
+// of the last-level cache (statistics and gradient of 128 MB at a time) is no
+// faster than one from memory: 660 us.
+template <typename T, int VPT, bool JOIN>
 __global__ __launch_bounds__(kThreads) void distill_grad(DistillArgs a) {
-  constexpr int N = Elem<T>::kN, VPT = EPT / N;
-  __shared__ EntryLds lds;
-  const int tid = threadIdx.x;
-  const int64_t nv = a.V / N, tasks = a.n * a.S;
+  const Walk wk = a.wk;
+  const int64_t tasks = a.n * wk.S;
   for (int64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
-    const int64_t row = t / a.S, seg = t - row * a.S;
-    const T* z = static_cast<const T*>(a.z) + row * a.ld;
+    const int64_t row = t / wk.S;
+    const int seg = (int)(t - row * wk.S);
+    const Row<T> z(a.z, a.ld, row, wk.V);
     T* out = static_cast<T*>(a.out) + row * a.ldo;
-    const int64_t v0 = seg * kThreads * VPT, tail_col = nv * N + tid;
-    const bool has_tail = seg == a.S - 1 && tail_col < a.V;
-    const float wt = (a.weight ? a.weight[row] : 1.f) * a.inv_t;
-    const float Z = a.stat[row * 4 + 1], tm = a.stat[row * 4 + 2], ts = a.stat[row * 4 + 3];
-    if (wt == 0.f || ts == 0.f) {   // (uniform) nothing flows into this row
-      const float zero[N] = {};
-#pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        const int64_t v = v0 + j * kThreads + tid;
-        if (v < nv) store_vec(out + v * N, Elem<T>::pack(zero));
-      }
-      if (has_tail) out[tail_col] = Elem<T>::cast(0.f);
+    const float wt = (a.weight ? a.weight[row] : 1.f) * a.inv_t, ts = a.stat[row * 4 + 3];
+    if (wt == 0.f || ts == 0.f) {   // nothing flows into this row
+      zero_segment<T, VPT>(z, out, wk, seg);
       continue;
     }
-    const Origin o(a.stat[row * 4], a.c);
-    const float scale = Z == 0.f ? 0.f : wt / Z;
-    u32x4 r[VPT];
+    const Segment<T, VPT> part(z, wk, seg);
+    RowStat st;
+    if (JOIN) st = join_parts(a.part + row * a.S, a.S, a.c);
+    else st = RowStat{a.stat[row * 4], a.stat[row * 4 + 1], 0.f};
+    const float o = origin(st.m), scale = ts != ts ? ts : st.z == 0.f ? 0.f : wt / st.z;
+    part.write(z, out, wk, seg, [&](float* x, int, auto n) {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int64_t v = v0 + j * kThreads + tid;
-      if (v < nv) r[j] = load_vec(z + v * N);
-    }
-    auto write = [&](auto big) {
-      auto grad = [&](float x) {
-        return __builtin_amdgcn_exp2f(shifted<decltype(big)::value>(x, o.m, o.mc, a.c)) * scale;
-      };
-#pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        const int64_t v = v0 + j * kThreads + tid;
-        if (v >= nv) break;
-        float x[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = grad(Elem<T>::get(r[j], i));
-        store_vec(out + v * N, Elem<T>::pack(x));
-      }
-      if (has_tail) out[tail_col] = Elem<T>::cast(grad(Elem<T>::load(z + tail_col)));
-    };
-    if (o.big) write(std::true_type()); else write(std::false_type());
-    const int64_t lo = v0 * N, whole = lo + (int64_t)kThreads * EPT;
-    distill_entries<T>(a, row, lo, seg == a.S - 1 ? a.V : whole, o, scale, wt, tm, ts, out, lds);
-    __syncthreads();
+      for (int k = 0; k < decltype(n)::value; ++k) x[k] = exp2_of(x[k], o, a.c) * scale;
+    });
   }
 }
 
-// ---- launches -------------------------------------------------------------------
+// A wave a row.  LOSS: the loss and the row's statistics.  With an output, what
+// distill_grad left at the teacher's entries is replaced by w (q - p) / T, the
+// p of equal columns summed in their order, rounded once.
+template <typename T, bool LOSS>
+__global__ __launch_bounds__(kThreads) void distill_finish(DistillArgs a) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.n; row += (int64_t)gridDim.x * 4) {
+    // what does not depend on the row pointer is on its way while that is read
+    const float tm = a.stat[row * 4 + 2], ts = a.stat[row * 4 + 3], wt = (a.weight ? a.weight[row] : 1.f) * a.inv_t;
+    int64_t b, e;
+    a.t.range(row, b, e);
+    // a lane's entry of the first 64 (most rows have no more) is read once
+    const bool has = b + lane < e;
+    const int32_t col0 = has ? a.t.col[b + lane] : -1;
+    const float val0 = has ? a.t.at(b + lane) : 0.f, x0 = has ? a.picked[b + lane] : 0.f;
+    auto entry = [&](int64_t i, int32_t& col, float& val) {
+      const bool first = i == b + lane;
+      col = first ? col0 : i < e ? a.t.col[i] : -1;
+      val = first ? val0 : i < e ? a.t.at(i) : 0.f;
+    };
+    const float l2t = log2_of(ts);
+    RowStat st;
+    if (LOSS) {
+      st = join_parts(a.part + row * a.S, a.S, a.c);
+      const float o = origin(st.m), l2z = log2_of(st.z);
+      float loss = 0.f;
+      for (int64_t i = b + lane; i < e; i += 64) {
+        int32_t col;
+        float val;
+        entry(i, col, val);
+        if (col < 0 || col >= a.V) continue;
+        const float u = (val - tm) * a.c - l2t, p = __builtin_amdgcn_exp2f(u), x = i == b + lane ? x0 : a.picked[i];
+        if (!(p == 0.f)) loss += p * (kLn2 * u - ((x - o) * a.inv_t - kLn2 * l2z));
+      }
+      loss = wave_sum(loss);
+      if (ts != ts) loss = st.z = ts;   // a column outside the vocabulary, or a NaN
+      if (lane == 0) {
+        a.loss[row] = ts == 0.f ? 0.f : loss;   // (no mass: nothing to learn)
+        a.stat[row * 4] = st.m;
+        a.stat[row * 4 + 1] = st.z;
+      }
+    } else {
+      st = RowStat{a.stat[row * 4], a.stat[row * 4 + 1], 0.f};
+    }
+    if (!a.out || wt == 0.f || ts == 0.f) continue;
+    const float o = origin(st.m), scale = st.z == 0.f ? 0.f : wt / st.z;
+    T* out = static_cast<T*>(a.out) + row * a.ldo;
+    for (int64_t base = b; base < e; base += 64) {
+      const int64_t i = base + lane;
+      int32_t mine, col;
+      float val;
+      entry(i, mine, val);
+      bool first = mine >= 0 && mine < a.V;
+      float p = 0.f;
+      for (int64_t from = b; from < e; from += 64) {
+        entry(from + lane, col, val);
+        const float share = col != -1 ? __builtin_amdgcn_exp2f((val - tm) * a.c - l2t) : 0.f;
+        const int count = (int)(e - from < 64 ? e - from : 64);
+        for (int j = 0; j < count; ++j) {
+          const bool same = (int32_t)__builtin_amdgcn_readlane((uint32_t)col, j) == mine;
+          first = first && !(same && from + j < i);
+          const float share_j = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(share), j));
+          p += same ? share_j : 0.f;
+        }
+      }
+      if (first) out[mine] = Elem<T>::cast(exp2_of(base == b ? x0 : a.picked[i], o, a.c) * scale - wt * p);
+    }
+  }
+}
 
-// Elements a thread holds.
-int elems_of(int64_t V) { return V <= 2048 ? 8 : V <= 4096 ? 16 : V <= 8192 ? 32 : 64; }
-int64_t segments(int64_t V, int type, int ept) {
-  const int64_t N = type == kF32 ? 4 : 8, nv = V / N, per = (int64_t)kThreads * (ept / N);
-  const int64_t s = (nv + per - 1) / per;
-  return s < 1 ? 1 : s;
+// ---- launches -----------------------------------------------------------------------
+
+// Pages a workgroup holds: as many as `most`, fewer in short rows, and fewer
+// where the workgroups would not fill the chip.
+struct Plan {
+  Walk wk;
+  int vpt;
+};
+Plan plan(int64_t n, int64_t V, int type, int most) {
+  const int64_t pages = (V / (type == kF32 ? 4 : 8) + kThreads - 1) / kThreads;
+  Plan p;
+  p.vpt = most;
+  while (p.vpt > 1 && p.vpt / 2 >= pages) p.vpt /= 2;
+  for (;; p.vpt /= 2) {
+    const int64_t step = pages > p.vpt ? 8 : 1, span = step * p.vpt, S = (pages + span - 1) / span * step;
+    p.wk = Walk{V, S < 1 ? 1 : S, (int)step};
+    if (p.vpt == 1 || n * p.wk.S >= kFill) return p;
+  }
 }
 bool sizes_ok(int64_t n, int64_t V, int type) {
   return n >= 0 && V >= 1 && V < (1ll << 31) - 4096 && type >= 0 && type <= 2 && n < (1ll << 40);
 }
 
-template <typename F>
-void with_ept(int ept, F&& f) {
-  if (ept == 8) f(std::integral_constant<int, 8>());
-  else if (ept == 16) f(std::integral_constant<int, 16>());
-  else if (ept == 32) f(std::integral_constant<int, 32>());
-  else f(std::integral_constant<int, 64>());
+template <int MOST, typename F>
+void with_vpt(int vpt, F&& f) {
+  if constexpr (MOST > 1)
+    if (vpt < MOST) return with_vpt<MOST / 2>(vpt, f);
+  f(std::integral_constant<int, MOST>());
+}
+
+// Threads a group whose maximum is kept for the alternatives: as many as leave
+// 16 k groups and 512 in the row, or as few as 1024 groups (a wave's registers)
+// allow.  Fewer groups are searched faster, smaller ones are read again faster.
+int group_lanes(int64_t S, int k) {
+  const int64_t least = 16 * k > 512 ? 16 * k : 512;
+  int lanes = 64;
+  while (lanes > 1) {
+    const int next = lanes == 64 ? 16 : lanes / 2;
+    if (S * kThreads / lanes >= least || S * kThreads / next > 64 * kKeyRegs) break;
+    lanes = next;
+  }
+  return lanes;
 }
 
 }  // namespace
@@ -658,30 +804,31 @@ void with_ept(int ept, F&& f) {
 // bytes of workspace of spmm_token_logprobs (k >= 0) and of the distillation (k = 0)
 SPMM_EXPORT int64_t spmm_vocab_ws(int64_t n, int64_t V, int type, int k) {
   if (!sizes_ok(n, V, type) || k < 0 || k > kMaxTop || k > V) return -1;
-  const int64_t S = segments(V, type, elems_of(V));
-  return n * S * (int64_t)(sizeof(Part) + k * sizeof(uint64_t));
+  const int64_t S = plan(n, V, type, kStatsPages).wk.S;
+  return n * S * (int64_t)(sizeof(Part) + (k ? kThreads / group_lanes(S, k) * sizeof(uint32_t) : 0));
 }
 
 SPMM_EXPORT int spmm_token_logprobs(const void* z, int64_t ld, int64_t n, int64_t V, int type, const void* tok, int wide,
-                                    int k, float c, float inv_t, float* logprob, float* entropy, float* stat, int64_t* rowptr,
-                                    int32_t* top_col, float* top_val, void* ws, int64_t ws_bytes, hipStream_t s) {
+                                    int k, float c, float inv_t, float* stat, int64_t* rowptr, int32_t* top_col,
+                                    float* top_val, void* ws, int64_t ws_bytes, hipStream_t s) {
   const int64_t need = spmm_vocab_ws(n, V, type, k);
   if (need < 0 || ws_bytes < need) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
-  const int ept = elems_of(V);
-  const int64_t S = segments(V, type, ept);
+  const Plan p = plan(n, V, type, kStatsPages);
+  const int64_t S = p.wk.S;
   Part* part = static_cast<Part*>(ws);
-  uint64_t* lists = reinterpret_cast<uint64_t*>(part + n * S);
-  const StatsArgs sa{z, ld, n, V, S, c, part, k, lists};
-  const JoinArgs ja{z, ld, n, V, S, c, inv_t, part, tok, wide, k, lists, logprob, entropy, stat, rowptr, top_col, top_val};
+  uint32_t* keys = reinterpret_cast<uint32_t*>(part + n * S);
+  const int lanes = group_lanes(S, k);
+  const StatsArgs sa{z, ld, n, p.wk, c, part, keys, lanes};
+  const JoinArgs ja{z, ld, n, p.wk, p.vpt, c, inv_t, part, tok, wide, k, lanes, keys, stat, rowptr, top_col, top_val};
   SPMM_VOCAB_TYPE(type, T, {
-    with_ept(ept, [&](auto e) {
+    with_vpt<kStatsPages>(p.vpt, [&](auto e) {
       constexpr int E = decltype(e)::value;
-      if (k) hipLaunchKernelGGL((vocab_stats<T, E, true, true>), dim3(groups_of(n * S)), dim3(kThreads), 0, s, sa);
-      else hipLaunchKernelGGL((vocab_stats<T, E, true, false>), dim3(groups_of(n * S)), dim3(kThreads), 0, s, sa);
+      if (k) hipLaunchKernelGGL((vocab_stats<T, E, true>), dim3(groups_of(n * S)), dim3(kThreads), 0, s, sa);
+      else hipLaunchKernelGGL((vocab_stats<T, E, false>), dim3(groups_of(n * S)), dim3(kThreads), 0, s, sa);
     });
     SPMM_LAUNCH_CHECK();
-    if (k) hipLaunchKernelGGL((vocab_join<T, true>), dim3(groups_of(n)), dim3(kThreads), 0, s, ja);
+    if (k) hipLaunchKernelGGL((vocab_join<T, true>), dim3(groups_of((n + 3) / 4)), dim3(kThreads), 0, s, ja);
     else hipLaunchKernelGGL((vocab_join<T, false>), dim3(groups_of((n + 3) / 4)), dim3(kThreads), 0, s, ja);
     SPMM_LAUNCH_CHECK();
   });
@@ -689,18 +836,18 @@ SPMM_EXPORT int spmm_token_logprobs(const void* z, int64_t ld, int64_t n, int64_
 }
 
 SPMM_EXPORT int spmm_token_logprobs_grad(const void* z, int64_t ld, int64_t n, int64_t V, int type, const void* tok,
-                                         int wide, float c, float inv_t, const float* stat, const float* entropy,
-                                         const float* g, const float* h, void* out, int64_t ldo, hipStream_t s) {
+                                         int wide, float c, float inv_t, const float* stat, const float* g,
+                                         const float* h, void* out, int64_t ldo, hipStream_t s) {
   if (!sizes_ok(n, V, type)) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
-  const int ept = elems_of(V);
-  const int64_t S = segments(V, type, ept);
-  const TokenGradArgs a{z, ld, n, V, S, c, inv_t, tok, wide, stat, entropy, g, h, out, ldo};
+  const Plan p = plan(n, V, type, kGradPages);
+  const TokenGradArgs a{z, ld, n, p.wk, c, inv_t, tok, wide, stat, g, h, out, ldo};
   SPMM_VOCAB_TYPE(type, T, {
-    with_ept(ept, [&](auto e) {
+    with_vpt<kGradPages>(p.vpt, [&](auto e) {
       constexpr int E = decltype(e)::value;
-      if (h) hipLaunchKernelGGL((vocab_token_grad<T, E, true>), dim3(groups_of(n * S)), dim3(kThreads), 0, s, a);
-      else hipLaunchKernelGGL((vocab_token_grad<T, E, false>), dim3(groups_of(n * S)), dim3(kThreads), 0, s, a);
+      const dim3 grid(groups_of(n * p.wk.S));
+      if (h) hipLaunchKernelGGL((vocab_token_grad<T, E, true>), grid, dim3(kThreads), 0, s, a);
+      else hipLaunchKernelGGL((vocab_token_grad<T, E, false>), grid, dim3(kThreads), 0, s, a);
     });
     SPMM_LAUNCH_CHECK();
   });
@@ -715,19 +862,22 @@ SPMM_EXPORT int spmm_distill(const void* z, int64_t ld, int64_t n, int64_t V, in
   const int64_t need = spmm_vocab_ws(n, V, type, 0);
   if (need < 0 || ws_bytes < need || val_type < 0 || val_type > 2) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
-  const int ept = elems_of(V);
-  const int64_t S = segments(V, type, ept);
+  const Plan p = plan(n, V, type, kStatsPages), q = plan(n, V, type, kGradPages);
   Part* part = static_cast<Part*>(ws);
-  const StatsArgs sa{z, ld, n, V, S, c, part, 0, nullptr};
-  const DistillArgs a{z, ld, n, V, S, c, inv_t, part, Teacher{rowptr, col, val, val_type, nnz}, loss, stat, picked,
-                      weight, out, ldo};
+  const StatsArgs sa{z, ld, n, p.wk, c, part, nullptr, 1};
+  const DistillArgs a{z, ld, n, V, q.wk, c, inv_t, part, p.wk.S, Teacher{rowptr, col, val, val_type, nnz}, loss, stat,
+                      picked, weight, out, ldo};
   SPMM_VOCAB_TYPE(type, T, {
-    with_ept(ept, [&](auto e) {
+    with_vpt<kStatsPages>(p.vpt, [&](auto e) {
       constexpr int E = decltype(e)::value;
-      hipLaunchKernelGGL((vocab_stats<T, E, false, false>), dim3(groups_of(n * S)), dim3(kThreads), 0, s, sa);
-      hipLaunchKernelGGL((distill_join<T>), dim3(groups_of((n + 3) / 4)), dim3(kThreads), 0, s, a);
-      if (out) hipLaunchKernelGGL((distill_grad<T, E>), dim3(groups_of(n * S)), dim3(kThreads), 0, s, a);
+      hipLaunchKernelGGL((distill_stats<T, E>), dim3(groups_of(n * p.wk.S + (n + 3) / 4)), dim3(kThreads), 0, s, sa, a);
     });
+    if (out)
+      with_vpt<kGradPages>(q.vpt, [&](auto e) {
+        constexpr int E = decltype(e)::value;
+        hipLaunchKernelGGL((distill_grad<T, E, true>), dim3(groups_of(n * q.wk.S)), dim3(kThreads), 0, s, a);
+      });
+    hipLaunchKernelGGL((distill_finish<T, true>), dim3(groups_of((n + 3) / 4)), dim3(kThreads), 0, s, a);
     SPMM_LAUNCH_CHECK();
   });
   return 0;
@@ -740,14 +890,15 @@ SPMM_EXPORT int spmm_distill_grad(const void* z, int64_t ld, int64_t n, int64_t 
                                   hipStream_t s) {
   if (!sizes_ok(n, V, type) || val_type < 0 || val_type > 2) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
-  const int ept = elems_of(V);
-  const DistillArgs a{z, ld, n, V, segments(V, type, ept), c, inv_t, nullptr, Teacher{rowptr, col, val, val_type, nnz},
-                      nullptr, const_cast<float*>(stat), const_cast<float*>(picked), weight, out, ldo};
+  const Plan q = plan(n, V, type, kGradPages);
+  const DistillArgs a{z, ld, n, V, q.wk, c, inv_t, nullptr, 0, Teacher{rowptr, col, val, val_type, nnz}, nullptr,
+                      const_cast<float*>(stat), const_cast<float*>(picked), weight, out, ldo};
   SPMM_VOCAB_TYPE(type, T, {
-    with_ept(ept, [&](auto e) {
+    with_vpt<kGradPages>(q.vpt, [&](auto e) {
       constexpr int E = decltype(e)::value;
-      hipLaunchKernelGGL((distill_grad<T, E>), dim3(groups_of(n * a.S)), dim3(kThreads), 0, s, a);
+      hipLaunchKernelGGL((distill_grad<T, E, false>), dim3(groups_of(n * q.wk.S)), dim3(kThreads), 0, s, a);
     });
+    hipLaunchKernelGGL((distill_finish<T, false>), dim3(groups_of((n + 3) / 4)), dim3(kThreads), 0, s, a);
     SPMM_LAUNCH_CHECK();
   });
   return 0;

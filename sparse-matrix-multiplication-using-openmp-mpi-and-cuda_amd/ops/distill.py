@@ -12,7 +12,8 @@ row -- e.g. ``token_logprobs(...).top``.  With temperature tau,
 * A row without entries, without mass (all -inf) or of weight 0 has a zero
   gradient; without entries or mass its loss is 0 too.
 * Column -1 marks an absent entry (a row padded to a fixed length); entries of
-  equal columns add up.  A column outside the vocabulary makes its row NaN.
+  equal columns add up.  A column outside the vocabulary, or a value of NaN or
+  +inf, makes its row NaN.
 * Masked student logits (-inf) have q = 0: the loss is +inf where the teacher
   has mass there.
 * Sums are held in fp32; results are the same in every run.

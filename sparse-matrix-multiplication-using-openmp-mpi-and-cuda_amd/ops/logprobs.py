@@ -34,9 +34,9 @@ from .csr import CSR
 
 _native.register_hip("spmm_vocab_ws", C.c_int64, C.c_int64, C.c_int, C.c_int, restype=C.c_int64)
 _native.register_hip("spmm_token_logprobs", c_vp, C.c_int64, C.c_int64, C.c_int64, C.c_int, c_vp, C.c_int, C.c_int,
-                     C.c_float, C.c_float, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, C.c_int64, c_vp)
-_native.register_hip("spmm_token_logprobs_grad", c_vp, C.c_int64, C.c_int64, C.c_int64, C.c_int, c_vp, C.c_int,
                      C.c_float, C.c_float, c_vp, c_vp, c_vp, c_vp, c_vp, C.c_int64, c_vp)
+_native.register_hip("spmm_token_logprobs_grad", c_vp, C.c_int64, C.c_int64, C.c_int64, C.c_int, c_vp, C.c_int,
+                     C.c_float, C.c_float, c_vp, c_vp, c_vp, c_vp, C.c_int64, c_vp)
 
 MAX_TOP = 128   # vocab_logits.hip kMaxTop
 LOG2E = 1.0 / math.log(2.0)
@@ -46,7 +46,7 @@ LOG2E = 1.0 / math.log(2.0)
 class TokenLogprobs:
     logprob: torch.Tensor    # fp32 [n]
     entropy: torch.Tensor    # fp32 [n]
-    stat: torch.Tensor       # fp32 [2, n]: the row's maximum m and sum of exp((z - m) / T)
+    stat: torch.Tensor       # fp32 [4, n]: both, the row's maximum m and its sum of exp((z - m) / T)
     temperature: float
     top: Optional[CSR]       # n x V, k entries a row, largest first (fp32 log-probabilities)
 
@@ -84,8 +84,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     k = int(k)
     if not 0 <= k <= min(MAX_TOP, V):
         raise ValueError(f"k must be between 0 and {min(MAX_TOP, V)}, got {k}")
-    stat = torch.empty((2, n), dtype=torch.float32, device=dev)
-    logprob, entropy = torch.empty((2, n), dtype=torch.float32, device=dev).unbind(0)
+    stat = torch.empty((4, n), dtype=torch.float32, device=dev)
+    logprob, entropy, _, _ = stat.unbind(0)
     top = None
     if k:
         top = CSR(n, V, torch.empty(n + 1, dtype=torch.int64, device=dev),
@@ -100,7 +100,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     if dev.type != "cuda":
         zf, t = z.float().contiguous(), tok.to(torch.int64)
         _native.check(_native.host().spmm_cpu_token_logprobs(
-            n, V, P(zf), P(t), inv_t, k, P(logprob), P(entropy), P(stat), P(top.col) if k else None,
+            n, V, P(zf), P(t), inv_t, k, P(stat), P(top.col) if k else None,
             P(top.val) if k else None, 0), "cpu_token_logprobs")
         return res
     lib = _native.hip()
@@ -109,8 +109,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     with R.on(dev):
         ws = torch.empty(bytes_, dtype=torch.uint8, device=dev)
         _native.check(lib.spmm_token_logprobs(
-            P(z), z.stride(0), n, V, code, P(tok), tok.dtype == torch.int64, k, LOG2E * inv_t, inv_t, P(logprob),
-            P(entropy), P(stat), P(top.rowptr) if k else None, P(top.col) if k else None, P(top.val) if k else None,
+            P(z), z.stride(0), n, V, code, P(tok), tok.dtype == torch.int64, k, LOG2E * inv_t, inv_t, P(stat),
+            P(top.rowptr) if k else None, P(top.col) if k else None, P(top.val) if k else None,
             P(ws), bytes_, _native.stream_ptr(dev)), "token_logprobs")
     return res
 
@@ -143,13 +143,13 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: Token
     if dev.type != "cuda":
         zf, t = z.float().contiguous(), tok.to(torch.int64)
         acc = torch.empty((n, V), dtype=torch.float32)
-        _native.check(_native.host().spmm_cpu_token_logprobs_grad(n, V, P(zf), P(t), inv_t, P(stats.entropy), P(g),
+        _native.check(_native.host().spmm_cpu_token_logprobs_grad(n, V, P(zf), P(t), inv_t, P(stats.stat), P(g),
                                                                   P(h), P(acc), 0), "cpu_token_logprobs_grad")
         out.copy_(acc)
         return out
     with R.on(dev):
         _native.check(_native.hip().spmm_token_logprobs_grad(
             P(z), z.stride(0), n, V, R.TYPES[z.dtype], P(tok), tok.dtype == torch.int64, LOG2E * inv_t, inv_t,
-            P(stats.stat), P(stats.entropy), P(g), P(h), P(out), out.stride(0), _native.stream_ptr(dev)),
+            P(stats.stat), P(g), P(h), P(out), out.stride(0), _native.stream_ptr(dev)),
             "token_logprobs_grad")
     return out

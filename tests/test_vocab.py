@@ -299,6 +299,26 @@ def test_logprobs_masks_and_ties(dev, dtype, V):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_logprobs_long_rows_of_ties_and_infinities(dev, dtype):
+    """More candidates than are ranked at once, fewer logits than alternatives, infinities beside other bits of a word."""
+    V = 131072 + 3
+    z, tok = logits(8, V, dtype, seed=5)
+    z[0] = 1.25
+    z[1] = -math.inf
+    z[1, ::40000] = torch.tensor([1.0, -2.0, 3.0, 0.0]).to(dtype)
+    z[2] = (z[2].float() * 0.25).round().to(dtype)
+    z[3, 70001], z[3, 70000] = math.inf, -1.5
+    z[4, 5], z[4, 4] = math.nan, -1.5
+    z[5] = torch.linspace(-9, 9, V).to(dtype)
+    z[6, :-2] = -math.inf
+    z[7] = math.nan
+    tok[1], tok[6] = 40000, V - 1
+    for k in (1, 20, 64, 128):
+        check_logprobs(z, tok, k, 1.0, dev)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_logprobs_layouts(dev):
     z, tok = logits(6, 501, torch.bfloat16, seed=2)
     wide = torch.zeros(6, 600, dtype=torch.bfloat16, device=dev)
@@ -417,7 +437,7 @@ def ref_distill(z, T, tau, w):
     for i in range(n):
         c, v = T.col.cpu()[ptr[i]:ptr[i + 1]].long(), T.val.cpu()[ptr[i]:ptr[i + 1]].double()
         c, v = c[c != -1], v[c != -1]
-        if ((c < 0) | (c >= V)).any():
+        if ((c < 0) | (c >= V)).any() or v.isnan().any() or (v == math.inf).any():
             loss[i], grad[i] = math.nan, (0.0 if w[i] == 0 else math.nan)
             continue
         if c.numel() == 0 or (v == -math.inf).all():
@@ -478,7 +498,7 @@ def test_distill_many_rows(dtype, n, V):
 @pytest.mark.parametrize("dev", DEVICES)
 def test_distill_rows(dev):
     V = 3000
-    z, _ = logits(14, V, torch.float32, seed=16)
+    z, _ = logits(16, V, torch.float32, seed=16)
     inf = math.inf
     rows = [[],                                             # no entry
             [(5, -inf), (6, -inf)],                         # no mass
@@ -493,12 +513,14 @@ def test_distill_rows(dev):
             [(1, 1.0), (2, 1.0)],                           # the student masks one of them
             [(1, 1.0), (2, 1.0)],                           # the student masks everything
             [(11, 2.0), (12, 1.0)],
+            [(11, 2.0), (12, math.nan)],
+            [(11, inf), (12, 0.0)],
             [(j * 2, float(j % 7)) for j in range(1400)]]   # more entries than are staged at once
     z[10, 2] = -inf
     z[11] = -inf
     z[0] = math.nan                                          # garbage in a row that is not trained on
     z[12, 5:11] = -inf
-    w = torch.linspace(0.5, 2.0, 14)
+    w = torch.linspace(0.5, 2.0, 16)
     w[12] = 0.0
     dz = check_distill(z, teacher_of(rows, V), 1.2, w, dev)
     assert (dz[0] == 0).all() and (dz[12] == 0).all()
