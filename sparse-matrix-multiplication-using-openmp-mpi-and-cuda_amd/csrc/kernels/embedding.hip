@@ -21,7 +21,9 @@ namespace {
 // ---- lookup -----------------------------------------------------------------
 constexpr int kLookupVecs = 4;   // loads in flight a lane
 
-template <typename T, int LPR>   // LPR lanes a row slice of LPR * kLookupVecs vectors
+// LPR lanes a row slice of LPR * kLookupVecs vectors.  STREAM: an output of over
+// 16 MB leaves the table's rows in the caches (32768 x 4096 bf16: 65 us instead of 77).
+template <typename T, int LPR, bool STREAM>
 __global__ __launch_bounds__(256) void embed_lookup(const T* __restrict__ W, int64_t ldw, int64_t V, int64_t D,
                                                     const void* __restrict__ tok, int wide, int64_t n, float scale,
                                                     T* __restrict__ Y, int64_t ldy, int64_t slices) {
@@ -30,7 +32,9 @@ __global__ __launch_bounds__(256) void embed_lookup(const T* __restrict__ W, int
   const int lane = threadIdx.x % LPR;
   const int64_t nv = D / N, tasks = n * slices;
   for (int64_t t = (int64_t)blockIdx.x * kGroups + threadIdx.x / LPR; t < tasks; t += (int64_t)gridDim.x * kGroups) {
-    const int64_t i = t / slices, s = t - i * slices;
+    // (a 64-bit division costs as much as the copy of a short row)
+    const int64_t i = tasks <= 0xffffffffll ? (int64_t)((uint32_t)t / (uint32_t)slices) : t / slices;
+    const int64_t s = t - i * slices;
     const int64_t id = token_at(tok, wide, i);
     const bool inside = id >= 0 && id < V;
     const float fill = id == -1 ? 0.f : __builtin_nanf("");   // padding, or a token that the table does not have
@@ -49,7 +53,8 @@ __global__ __launch_bounds__(256) void embed_lookup(const T* __restrict__ W, int
       float x[N];
 #pragma unroll
       for (int e = 0; e < N; ++e) x[e] = inside ? Elem<T>::get(r[u], e) * scale : fill;
-      store_vec(y + (v0 + u * LPR) * N, Elem<T>::pack(x));
+      T* to = y + (v0 + u * LPR) * N;
+      if (STREAM) stream_vec(to, Elem<T>::pack(x)); else store_vec(to, Elem<T>::pack(x));
     }
     const int64_t c = nv * N + lane;   // the last D % N columns (N <= LPR)
     if (s == slices - 1 && c < D) y[c] = Elem<T>::cast(inside ? Elem<T>::load(w + c) * scale : fill);
@@ -64,8 +69,10 @@ int lookup(const T* W, int64_t ldw, int64_t V, int64_t D, const void* tok, int w
     constexpr int L = decltype(lpr)::value;
     const int64_t slices = nv > 0 ? (nv + L * kLookupVecs - 1) / (L * kLookupVecs) : 1;
     const int64_t groups = (n * slices + 256 / L - 1) / (256 / L);
-    hipLaunchKernelGGL((embed_lookup<T, L>), dim3(groups_of(groups)), dim3(256), 0, s, W, ldw, V, D, tok, wide, n,
-                       scale, Y, ldy, slices);
+    const bool stream = n * D * (int64_t)sizeof(T) >= kStreamBytes;
+    auto kernel = stream ? embed_lookup<T, L, true> : embed_lookup<T, L, false>;
+    hipLaunchKernelGGL(kernel, dim3(groups_of(groups)), dim3(256), 0, s, W, ldw, V, D, tok, wide, n, scale, Y, ldy,
+                       slices);
   };
   // the fewest lanes that still hold a row's vectors in one slice
   if (nv <= 8 * kLookupVecs) go(std::integral_constant<int, 8>());

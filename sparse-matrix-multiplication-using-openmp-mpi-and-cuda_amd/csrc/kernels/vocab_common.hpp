@@ -128,6 +128,15 @@ __device__ __forceinline__ void store_vec(T* p, const u32x4& v) {
   *reinterpret_cast<At*>(p) = v;
 }
 
+// The same past the caches' replacement order: for what is larger than the L2
+// caches and not read again soon.
+template <typename T>
+__device__ __forceinline__ void stream_vec(T* p, const u32x4& v) {
+  using At = std::conditional_t<sizeof(T) == 2, u32x4_at2, u32x4_at4>;
+  __builtin_nontemporal_store(v, reinterpret_cast<At*>(p));
+}
+constexpr int64_t kStreamBytes = 16 << 20;   // outputs that are written so
+
 // Reductions over a wave.  Lanes are paired inside rows of 16 by data-parallel
 // primitives (no LDS), the four rows by lane reads: the result is uniform.
 template <int CTRL>

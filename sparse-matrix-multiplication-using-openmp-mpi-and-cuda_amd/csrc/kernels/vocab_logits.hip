@@ -49,8 +49,10 @@ struct Row {
     head = head < V ? head : V;
     nv = (V - head) / N;
   }
+  // (past the caches' replacement order, as are the gradients' stores: a step over 4096 x 131072 bf16 502 us
+  // instead of 575; at 4 to 128 MB of logits the kernels take between 30 % less and 4 % more)
   __device__ __forceinline__ u32x4 vec(int v) const {
-    return *reinterpret_cast<const u32x4*>(z + head + (int64_t)v * N);
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(z + head + (int64_t)v * N));
   }
   __device__ __forceinline__ int col(int v) const { return head + v * N; }
   // column of extra element x of 2 N, or -1
@@ -239,10 +241,9 @@ struct JoinArgs {
 constexpr int kCand = 512;      // candidates of a row that are ranked against each other
 constexpr int kHits = 256;      // groups of a row that are read again
 constexpr int kKeyRegs = 16;    // groups of a row whose maxima a lane keeps
-constexpr int kFlight = 2;      // vectors of a lane that are read at a time (8: 13 KB of LDS a wave, half the waves)
+constexpr int kFlight = 4;      // vectors of a lane that are read at a time
 
 struct TopLds {   // of one wave
-  u32x4 vec[kFlight][64];
   uint64_t cand[kCand + 8];
   int hit[kHits];
 };
@@ -363,22 +364,18 @@ __device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& 
 #pragma unroll 1
     for (int i0 = 0; i0 < vecs; i0 += 64 * kFlight) {
       u32x4 x[kFlight];
+      int v[kFlight];
 #pragma unroll
       for (int f = 0; f < kFlight; ++f) {
-        const int v = place(i0 + f * 64 + lane);
-        x[f] = z.vec(v < 0 ? 0 : v);   // (there is a vector, or no group would be hit)
+        v[f] = place(i0 + f * 64 + lane);
+        x[f] = z.vec(v[f] < 0 ? 0 : v[f]);   // (there is a vector, or no group would be hit)
       }
 #pragma unroll
-      for (int f = 0; f < kFlight; ++f) s.vec[f][lane] = x[f];
-      wave_fence();
-#pragma unroll 1
-      for (int f = 0; f < kFlight && i0 + f * 64 < vecs; ++f) {
-        const int v = place(i0 + f * 64 + lane);
-        const u32x4 y = s.vec[f][lane];
+      for (int f = 0; f < kFlight; ++f) {
+        if (i0 + f * 64 >= vecs) break;
 #pragma unroll
-        for (int e = 0; e < N; ++e) offer(v >= 0, Elem<T>::get(y, e), z.col(v) + e);
+        for (int e = 0; e < N; ++e) offer(v[f] >= 0, Elem<T>::get(x[f], e), z.col(v[f]) + e);
       }
-      wave_fence();
     }
     {
       const int c = z.extra(lane);
@@ -498,7 +495,7 @@ struct Segment {
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] = Elem<T>::get(r[j], i);
       f(x, z.col(v), std::integral_constant<int, N>());
-      store_vec(out + z.col(v), Elem<T>::pack(x));
+      stream_vec(out + z.col(v), Elem<T>::pack(x));
     }
     if (extra >= 0) {
       float x[1] = {tail};
@@ -513,7 +510,7 @@ __device__ __forceinline__ void zero_segment(const Row<T>& z, T* out, const Walk
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int v = wk.page(seg, j, VPT) * kThreads + (int)threadIdx.x;
-    if (v < z.nv) store_vec(out + z.col(v), u32x4{0u, 0u, 0u, 0u});
+    if (v < z.nv) stream_vec(out + z.col(v), u32x4{0u, 0u, 0u, 0u});
   }
   const int extra = seg == 0 ? z.extra(threadIdx.x) : -1;
   if (extra >= 0) out[extra] = Elem<T>::cast(0.f);
@@ -653,12 +650,12 @@ __global__ __launch_bounds__(kThreads) void distill_stats(StatsArgs s, DistillAr
 // their segments'.
 //
 // Bytes bound a step of loss and gradient: the logits are read twice and the
-// gradient written once, 3.2 GB for 4096 x 131072 bf16 in 580 us (519 at the
+// gradient written once, 3.2 GB for 4096 x 131072 bf16 in 502 us (519 at the
 // rate of a large copy).  One read would take a row of 256 KB in registers
 // from its statistics to its gradient, half of a CU's: a workgroup a row with
-// half of it kept took 574 us, with all of it spilling 670.  A second read out
-// of the last-level cache (statistics and gradient of 128 MB at a time) is no
-// faster than one from memory: 660 us.
+// half of it kept took 574 us, with all of it spilling 670, where these kernels
+// then took 580.  A second read out of the last-level cache (statistics and
+// gradient of 128 MB at a time) is no faster than one from memory: 660 us.
 template <typename T, int VPT, bool JOIN>
 __global__ __launch_bounds__(kThreads) void distill_grad(DistillArgs a) {
   const Walk wk = a.wk;
