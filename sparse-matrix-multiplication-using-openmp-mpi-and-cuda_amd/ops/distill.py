@@ -45,62 +45,62 @@ _native.register_hip("spmm_distill_grad", c_vp, C.c_int64, C.c_int64, C.c_int64,
 @dataclass
 class DistillLoss:
     loss: torch.Tensor       # fp32 [n]
-    stat: torch.Tensor       # fp32 [n, 4]: student's maximum m and sum of exp((z - m) / tau), the teacher's two
-    picked: torch.Tensor     # fp32 [nnz]: the student's logits at the teacher's entries
+    saved: torch.Tensor      # fp32: loss; per row the student's maximum and sum, the teacher's two; the student's
+                             # logits at the teacher's entries; workspace
+    rows: int
+    entries: int
     temperature: float
 
 
-def _operands(logits: torch.Tensor, teacher: CSR) -> Tuple[torch.Tensor, torch.Tensor]:
+def _operands(logits: torch.Tensor, teacher: CSR):
     z = logits_rows(logits)
     n, V = z.shape
+    ptr, col, val = teacher.rowptr, teacher.col, teacher.val
     if teacher.m != n or teacher.n != V:
         raise ValueError(f"the teacher is {teacher.m} x {teacher.n}, the logits {n} x {V}")
-    R.same_device(z.device, **{"teacher.rowptr": teacher.rowptr, "teacher.col": teacher.col, "teacher.val": teacher.val})
-    if teacher.rowptr.dtype != torch.int64 or tuple(teacher.rowptr.shape) != (n + 1,):
-        raise ValueError(f"teacher.rowptr must be int64 [{n + 1}], got {teacher.rowptr.dtype} "
-                         f"{tuple(teacher.rowptr.shape)}")
-    if teacher.col.dtype != torch.int32 or teacher.col.dim() != 1:
-        raise ValueError(f"teacher.col must be int32 [nnz], got {teacher.col.dtype} {tuple(teacher.col.shape)}")
-    if teacher.val.dtype not in R.TYPES or teacher.val.shape != teacher.col.shape:
-        raise ValueError(f"teacher.val must be float32, bfloat16 or float16 [{teacher.nnz}], got {teacher.val.dtype} "
-                         f"{tuple(teacher.val.shape)}")
-    return z, CSR(n, V, teacher.rowptr.contiguous(), teacher.col.contiguous(), teacher.val.contiguous())
+    R.same_device(z.device, teacher=ptr, teacher_col=col, teacher_val=val)
+    if ptr.dtype != torch.int64 or ptr.dim() != 1 or ptr.shape[0] != n + 1:
+        raise ValueError(f"teacher.rowptr must be int64 [{n + 1}], got {ptr.dtype} {tuple(ptr.shape)}")
+    if col.dtype != torch.int32 or col.dim() != 1:
+        raise ValueError(f"teacher.col must be int32 [nnz], got {col.dtype} {tuple(col.shape)}")
+    if val.dtype not in R.TYPES or val.shape != col.shape:
+        raise ValueError(f"teacher.val must be float32, bfloat16 or float16 [{col.shape[0]}], got {val.dtype} "
+                         f"{tuple(val.shape)}")
+    return z, n, V, ptr.contiguous(), col.contiguous(), val.contiguous()
 
 
 def _run(logits, teacher, weight, temperature, out, gradient) -> Tuple[DistillLoss, Optional[torch.Tensor]]:
     R.no_grad_of("distill_loss_grad", logits, weight, out, teacher.val)
-    z, t = _operands(logits, teacher)
-    n, V = z.shape
-    dev = z.device
+    z, n, V, ptr, col, val = _operands(logits, teacher)
+    dev, nnz, code = z.device, col.shape[0], R.TYPES[z.dtype]
     R.same_device(dev, weight=weight)
     weight = R.per_row(weight, n, "weight")
     inv_t = R.inverse_temperature(temperature)
-    loss = torch.empty(n, dtype=torch.float32, device=dev)
-    stat = torch.empty((n, 4), dtype=torch.float32, device=dev)
-    picked = torch.empty(t.nnz, dtype=torch.float32, device=dev)
+    gpu = dev.type == "cuda"
+    ws = _native.hip().spmm_vocab_ws(n, V, code, 0) if gpu else 0
+    head = (5 * n + nnz + 3) // 4 * 4   # (the workspace starts at 16 bytes)
+    saved = torch.empty(head + ws // 4, dtype=torch.float32, device=dev)
+    res = DistillLoss(saved[:n], saved, n, nnz, float(temperature))
     if gradient:
         out = gradient_out(out, z)
-    res = DistillLoss(loss, stat, picked, float(temperature))
     if n == 0:
         return res, out
-    P = _native.ptr
-    if dev.type != "cuda":
-        zf, val = z.float().contiguous(), t.val.float()
+    at = saved.data_ptr()
+    w = weight.data_ptr() if weight is not None else None
+    if not gpu:
+        zf, vf = z.float().contiguous(), val.float()
         acc = torch.empty((n, V), dtype=torch.float32) if gradient else None
-        _native.check(_native.host().spmm_cpu_distill(n, V, P(zf), P(t.rowptr), P(t.col), P(val), t.nnz, inv_t, P(loss),
-                                                      P(stat), P(weight), P(acc), 0), "cpu_distill")
+        _native.check(_native.host().spmm_cpu_distill(
+            n, V, zf.data_ptr(), ptr.data_ptr(), col.data_ptr(), vf.data_ptr(), nnz, inv_t, at, at + 4 * n, w,
+            acc.data_ptr() if gradient else None, 0), "cpu_distill")
         if gradient:
             out.copy_(acc)
         return res, out
-    lib = _native.hip()
-    code = R.TYPES[z.dtype]
-    bytes_ = lib.spmm_vocab_ws(n, V, code, 0)
     with R.on(dev):
-        ws = torch.empty(bytes_, dtype=torch.uint8, device=dev)
-        _native.check(lib.spmm_distill(
-            P(z), z.stride(0), n, V, code, P(t.rowptr), P(t.col), P(t.val), R.TYPES[t.val.dtype], t.nnz, LOG2E * inv_t,
-            inv_t, P(loss), P(stat), P(picked), P(weight), P(out) if gradient else None,
-            out.stride(0) if gradient else 0, P(ws), bytes_, _native.stream_ptr(dev)), "distill")
+        _native.check(_native.hip().spmm_distill(
+            z.data_ptr(), z.stride(0), n, V, code, ptr.data_ptr(), col.data_ptr(), val.data_ptr(), R.TYPES[val.dtype],
+            nnz, LOG2E * inv_t, inv_t, at, at + 4 * n, at + 20 * n, w, out.data_ptr() if gradient else None,
+            out.stride(0) if gradient else 0, at + 4 * head, ws, _native.stream_ptr(dev)), "distill")
     return res, out
 
 
@@ -125,24 +125,23 @@ def distill_grad(logits: torch.Tensor, teacher: CSR, stats: DistillLoss, weight:
     loss: ``stats`` is what :func:`distill_loss` returned for the same logits
     and teacher.  ``out`` may be the logits themselves."""
     R.no_grad_of("distill_grad", logits, weight, out, teacher.val)
-    z, t = _operands(logits, teacher)
-    n, V = z.shape
-    dev = z.device
-    R.same_device(dev, weight=weight, stats=stats.stat)
+    z, n, V, ptr, col, val = _operands(logits, teacher)
+    dev, nnz = z.device, col.shape[0]
+    R.same_device(dev, weight=weight, stats=stats.saved)
     weight = R.per_row(weight, n, "weight")
-    if stats.stat.shape[0] != n or stats.picked.shape[0] != t.nnz:
-        raise ValueError(f"stats are of {stats.stat.shape[0]} rows and {stats.picked.shape[0]} entries, the operands "
-                         f"have {n} and {t.nnz}")
+    if stats.rows != n or stats.entries != nnz:
+        raise ValueError(f"stats are of {stats.rows} rows and {stats.entries} entries, the operands have {n} and {nnz}")
     inv_t = R.inverse_temperature(stats.temperature)
     out = gradient_out(out, z)
     if n == 0:
         return out
-    P = _native.ptr
     if dev.type != "cuda":
-        return _run(z, t, weight, stats.temperature, out, True)[1]
+        return _run(z, teacher, weight, stats.temperature, out, True)[1]
+    at = stats.saved.data_ptr()
     with R.on(dev):
         _native.check(_native.hip().spmm_distill_grad(
-            P(z), z.stride(0), n, V, R.TYPES[z.dtype], P(t.rowptr), P(t.col), P(t.val), R.TYPES[t.val.dtype], t.nnz,
-            LOG2E * inv_t, inv_t, P(stats.stat), P(stats.picked), P(weight), P(out), out.stride(0),
+            z.data_ptr(), z.stride(0), n, V, R.TYPES[z.dtype], ptr.data_ptr(), col.data_ptr(), val.data_ptr(),
+            R.TYPES[val.dtype], nnz, LOG2E * inv_t, inv_t, at + 4 * n, at + 20 * n,
+            weight.data_ptr() if weight is not None else None, out.data_ptr(), out.stride(0),
             _native.stream_ptr(dev)), "distill_grad")
     return out

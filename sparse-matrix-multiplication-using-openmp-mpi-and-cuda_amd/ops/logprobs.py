@@ -96,12 +96,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     res = TokenLogprobs(logprob, entropy, stat, float(temperature), top)
     if n == 0:
         return res
-    P = _native.ptr
+    at = (top.rowptr.data_ptr(), top.col.data_ptr(), top.val.data_ptr()) if k else (None, None, None)
     if dev.type != "cuda":
         zf, t = z.float().contiguous(), tok.to(torch.int64)
-        _native.check(_native.host().spmm_cpu_token_logprobs(
-            n, V, P(zf), P(t), inv_t, k, P(stat), P(top.col) if k else None,
-            P(top.val) if k else None, 0), "cpu_token_logprobs")
+        _native.check(_native.host().spmm_cpu_token_logprobs(n, V, zf.data_ptr(), t.data_ptr(), inv_t, k,
+                                                             stat.data_ptr(), at[1], at[2], 0), "cpu_token_logprobs")
         return res
     lib = _native.hip()
     code = R.TYPES[z.dtype]
@@ -109,9 +108,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     with R.on(dev):
         ws = torch.empty(bytes_, dtype=torch.uint8, device=dev)
         _native.check(lib.spmm_token_logprobs(
-            P(z), z.stride(0), n, V, code, P(tok), tok.dtype == torch.int64, k, LOG2E * inv_t, inv_t, P(stat),
-            P(top.rowptr) if k else None, P(top.col) if k else None, P(top.val) if k else None,
-            P(ws), bytes_, _native.stream_ptr(dev)), "token_logprobs")
+            z.data_ptr(), z.stride(0), n, V, code, tok.data_ptr(), tok.dtype == torch.int64, k, LOG2E * inv_t, inv_t,
+            stat.data_ptr(), *at, ws.data_ptr(), bytes_, _native.stream_ptr(dev)), "token_logprobs")
     return res
 
 
@@ -139,17 +137,19 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: Token
     out = gradient_out(out, z)
     if n == 0:
         return out
-    P = _native.ptr
+    at_g = g.data_ptr() if g is not None else None
+    at_h = h.data_ptr() if h is not None else None
     if dev.type != "cuda":
         zf, t = z.float().contiguous(), tok.to(torch.int64)
         acc = torch.empty((n, V), dtype=torch.float32)
-        _native.check(_native.host().spmm_cpu_token_logprobs_grad(n, V, P(zf), P(t), inv_t, P(stats.stat), P(g),
-                                                                  P(h), P(acc), 0), "cpu_token_logprobs_grad")
+        _native.check(_native.host().spmm_cpu_token_logprobs_grad(n, V, zf.data_ptr(), t.data_ptr(), inv_t,
+                                                                  stats.stat.data_ptr(), at_g, at_h, acc.data_ptr(), 0),
+                      "cpu_token_logprobs_grad")
         out.copy_(acc)
         return out
     with R.on(dev):
         _native.check(_native.hip().spmm_token_logprobs_grad(
-            P(z), z.stride(0), n, V, R.TYPES[z.dtype], P(tok), tok.dtype == torch.int64, LOG2E * inv_t, inv_t,
-            P(stats.stat), P(g), P(h), P(out), out.stride(0), _native.stream_ptr(dev)),
+            z.data_ptr(), z.stride(0), n, V, R.TYPES[z.dtype], tok.data_ptr(), tok.dtype == torch.int64, LOG2E * inv_t,
+            inv_t, stats.stat.data_ptr(), at_g, at_h, out.data_ptr(), out.stride(0), _native.stream_ptr(dev)),
             "token_logprobs_grad")
     return out
