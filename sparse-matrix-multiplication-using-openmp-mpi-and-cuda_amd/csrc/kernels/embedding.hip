@@ -377,6 +377,10 @@ struct Cols {
 #pragma unroll
     for (int b = 0; b < kVecs; ++b) v[b] = load_vec(row + from + b * Elem<T>::kN);
   }
+  __device__ __forceinline__ void fetch(const T* row, int64_t from) {   // what is read once
+#pragma unroll
+    for (int b = 0; b < kVecs; ++b) v[b] = fetch_vec(row + from + b * Elem<T>::kN);
+  }
   __device__ __forceinline__ float get(int e) const { return Elem<T>::get(v[e / Elem<T>::kN], e % Elem<T>::kN); }
 };
 
@@ -482,9 +486,10 @@ __global__ __launch_bounds__(256) void embed_grad_sum(GradArgs a) {
     for (int r0 = 0; r0 < cnt && __builtin_amdgcn_readlane(key, r0) < V; r0 += kFlight) {
       Cols<TI, N> x[kFlight];
 #pragma unroll
-      for (int u = 0; u < kFlight; ++u)   // (behind the last entry: that one again)
-        x[u].load(static_cast<const TI*>(a.dy) + (int64_t)__builtin_amdgcn_readlane(pos, r0 + u < cnt ? r0 + u : cnt - 1) * a.lddy,
-                  from);
+      for (int u = 0; u < kFlight; ++u) {   // (behind the last entry: that one again)
+        const int64_t i = __builtin_amdgcn_readlane(pos, r0 + u < cnt ? r0 + u : cnt - 1);
+        x[u].fetch(static_cast<const TI*>(a.dy) + i * a.lddy, from);
+      }
 #pragma unroll
       for (int u = 0; u < kFlight; ++u) {
         const int r = r0 + u;

@@ -135,6 +135,11 @@ __device__ __forceinline__ void stream_vec(T* p, const u32x4& v) {
   using At = std::conditional_t<sizeof(T) == 2, u32x4_at2, u32x4_at4>;
   __builtin_nontemporal_store(v, reinterpret_cast<At*>(p));
 }
+template <typename T>
+__device__ __forceinline__ u32x4 fetch_vec(const T* p) {
+  using At = std::conditional_t<sizeof(T) == 2, u32x4_at2, u32x4_at4>;
+  return __builtin_nontemporal_load(reinterpret_cast<const At*>(p));
+}
 constexpr int64_t kStreamBytes = 16 << 20;   // outputs that are written so
 
 // Reductions over a wave.  Lanes are paired inside rows of 16 by data-parallel
