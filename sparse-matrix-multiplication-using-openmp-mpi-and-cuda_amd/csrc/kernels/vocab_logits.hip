@@ -353,7 +353,7 @@ __device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& 
       if (((m >> lane) & 1) && at < kCand) s.cand[at] = entry_of(key_of(x), col);
       count += __popcll(m);
     };
-    const int vecs = hits << slots_log;
+    const int vecs = z.nv > 0 ? hits << slots_log : 0;   // (a short row may have extra elements alone)
     auto place = [&](int i) {   // vector i of the hits, or -1
       if (i >= vecs) return -1;
       const int g = s.hit[i >> slots_log], slot = i & ((1 << slots_log) - 1);
@@ -368,7 +368,7 @@ __device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& 
 #pragma unroll
       for (int f = 0; f < kFlight; ++f) {
         v[f] = place(i0 + f * 64 + lane);
-        x[f] = z.vec(v[f] < 0 ? 0 : v[f]);   // (there is a vector, or no group would be hit)
+        x[f] = z.vec(v[f] < 0 ? 0 : v[f]);
       }
 #pragma unroll
       for (int f = 0; f < kFlight; ++f) {

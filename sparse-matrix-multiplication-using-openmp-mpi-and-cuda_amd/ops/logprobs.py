@@ -91,8 +91,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
         top = CSR(n, V, torch.empty(n + 1, dtype=torch.int64, device=dev),
                   torch.empty(n * k, dtype=torch.int32, device=dev),
                   torch.empty(n * k, dtype=torch.float32, device=dev))
-        if n == 0 or dev.type != "cuda":
-            top.rowptr.copy_(torch.arange(0, n * k + 1, k))
+        if n == 0:
+            top.rowptr.zero_()
+        elif dev.type != "cuda":
+            torch.arange(0, n * k + 1, k, out=top.rowptr)
     res = TokenLogprobs(logprob, entropy, stat, float(temperature), top)
     if n == 0:
         return res

@@ -319,6 +319,19 @@ def test_logprobs_long_rows_of_ties_and_infinities(dev, dtype):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [3, 700, 20001])
+def test_logprobs_order_of_the_smallest(dev, dtype, V):
+    """Logits of a few of the type's smallest steps around zero, of both signs."""
+    f = torch.finfo(dtype)
+    step = f.smallest_normal * f.eps
+    z = (torch.randint(-3, 4, (4, V), generator=gen(24)).double() * step).to(dtype)
+    z[1] = -z[1].abs()
+    z[2, : V // 2] = -math.inf
+    check_logprobs(z, torch.randint(0, V, (4,), generator=gen(25)), min(V, 100), 1.0, dev)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_logprobs_layouts(dev):
     z, tok = logits(6, 501, torch.bfloat16, seed=2)
     wide = torch.zeros(6, 600, dtype=torch.bfloat16, device=dev)
