@@ -5,9 +5,11 @@
 #include <omp.h>
 
 #include <algorithm>
+#include <cerrno>
 #include <cmath>
 #include <cstdint>
 #include <limits>
+#include <new>
 #include <numeric>
 #include <vector>
 
@@ -19,6 +21,25 @@ constexpr double kNoMass = -std::numeric_limits<double>::infinity();
 const float kNan = std::numeric_limits<float>::quiet_NaN();
 
 inline int threads_or_default(int n) { return n > 0 ? n : omp_get_max_threads(); }
+
+// One scratch row of n elements for every thread, allocated before the threads
+// start: false (and no exception, which a C caller could not take) if there is
+// no memory for them.
+template <typename T>
+struct Scratch {
+  std::vector<T> rows;
+  size_t n = 0;
+  bool make(int threads, int64_t width) noexcept {
+    n = (size_t)width;
+    try {
+      rows.resize((size_t)threads * n);
+    } catch (const std::exception&) {
+      return false;
+    }
+    return true;
+  }
+  T* mine() { return rows.data() + (size_t)omp_get_thread_num() * n; }
+};
 
 // maximum of the numbers (a NaN is passed over; it reaches the sum), and the sum of exp((z - m) / T)
 struct RowSum {
@@ -67,57 +88,57 @@ SPMM_HOST_EXPORT int spmm_cpu_embedding(int64_t n, int64_t V, int64_t D, const f
 // dW (fp32, given) += scale * S^T dY
 SPMM_HOST_EXPORT int spmm_cpu_embedding_grad(int64_t n, int64_t V, int64_t D, const float* dY, const int64_t* tok,
                                              double scale, float* dW, int nthreads) {
-  std::vector<int64_t> pos;
-  pos.reserve((size_t)n);
-  for (int64_t i = 0; i < n; ++i)
-    if (tok[i] >= 0 && tok[i] < V) pos.push_back(i);
-  std::stable_sort(pos.begin(), pos.end(), [&](int64_t a, int64_t b) { return tok[a] < tok[b]; });
-  std::vector<int64_t> start;   // first of each run of equal tokens
-  for (size_t i = 0; i < pos.size(); ++i)
-    if (i == 0 || tok[pos[i]] != tok[pos[i - 1]]) start.push_back((int64_t)i);
-  start.push_back((int64_t)pos.size());
-#pragma omp parallel num_threads(threads_or_default(nthreads))
-  {
-    std::vector<double> acc((size_t)D);
-#pragma omp for schedule(dynamic, 16)
-    for (int64_t r = 0; r < (int64_t)start.size() - 1; ++r) {
-      std::fill(acc.begin(), acc.end(), 0.0);
-      for (int64_t i = start[(size_t)r]; i < start[(size_t)r + 1]; ++i) {
-        const float* x = dY + pos[(size_t)i] * D;
-        for (int64_t d = 0; d < D; ++d) acc[(size_t)d] += x[d];
-      }
-      float* w = dW + tok[pos[(size_t)start[(size_t)r]]] * D;
-      for (int64_t d = 0; d < D; ++d) w[d] = (float)(w[d] + acc[(size_t)d] * scale);
+  const int threads = threads_or_default(nthreads);
+  std::vector<int64_t> pos, start;   // positions by token; the first of each run of equal tokens
+  Scratch<double> scratch;
+  try {
+    for (int64_t i = 0; i < n; ++i)
+      if (tok[i] >= 0 && tok[i] < V) pos.push_back(i);
+    std::stable_sort(pos.begin(), pos.end(), [&](int64_t a, int64_t b) { return tok[a] < tok[b]; });
+    for (size_t i = 0; i < pos.size(); ++i)
+      if (i == 0 || tok[pos[i]] != tok[pos[i - 1]]) start.push_back((int64_t)i);
+    start.push_back((int64_t)pos.size());
+  } catch (const std::exception&) {
+    return ENOMEM;
+  }
+  if (!scratch.make(threads, D)) return ENOMEM;
+#pragma omp parallel for schedule(dynamic, 16) num_threads(threads)
+  for (int64_t r = 0; r < (int64_t)start.size() - 1; ++r) {
+    double* acc = scratch.mine();
+    std::fill(acc, acc + D, 0.0);
+    for (int64_t i = start[(size_t)r]; i < start[(size_t)r + 1]; ++i) {
+      const float* x = dY + pos[(size_t)i] * D;
+      for (int64_t d = 0; d < D; ++d) acc[d] += x[d];
     }
+    float* w = dW + tok[pos[(size_t)start[(size_t)r]]] * D;
+    for (int64_t d = 0; d < D; ++d) w[d] = (float)(w[d] + acc[d] * scale);
   }
   return 0;
 }
 
 // stat: [4][n] log-probability, entropy, maximum, Z.  top_col / top_val: [n][k].
 SPMM_HOST_EXPORT int spmm_cpu_token_logprobs(int64_t n, int64_t V, const float* z, const int64_t* tok, double inv_t,
-                                             int k, float* stat, int32_t* top_col,
-                                             float* top_val, int nthreads) {
-#pragma omp parallel num_threads(threads_or_default(nthreads))
-  {
-    std::vector<int32_t> idx((size_t)(k > 0 ? V : 0));
-#pragma omp for
-    for (int64_t i = 0; i < n; ++i) {
-      const float* zi = z + i * V;
-      const RowSum r = row_sum(zi, V, inv_t);
-      const double o = origin(r.m), logz = r.z == 0 ? 0.0 : std::log(r.z);
-      const int64_t t = tok[i];
-      stat[i] = t >= 0 && t < V ? (float)((zi[t] - o) * inv_t - logz) : (t == -1 ? 0.f : kNan);
-      stat[n + i] = r.z == 0 ? 0.f : (float)(logz - r.u / r.z);
-      stat[2 * n + i] = (float)r.m;
-      stat[3 * n + i] = (float)r.z;
-      if (k > 0) {
-        std::iota(idx.begin(), idx.end(), 0);
-        std::partial_sort(idx.begin(), idx.begin() + k, idx.end(),
-                          [&](int32_t a, int32_t b) { return before(zi, a, b); });
-        for (int j = 0; j < k; ++j) {
-          top_col[i * k + j] = idx[(size_t)j];
-          top_val[i * k + j] = (float)((zi[idx[(size_t)j]] - o) * inv_t - logz);
-        }
+                                             int k, float* stat, int32_t* top_col, float* top_val, int nthreads) {
+  const int threads = threads_or_default(nthreads);
+  Scratch<int32_t> scratch;
+  if (!scratch.make(threads, k > 0 ? V : 0)) return ENOMEM;
+#pragma omp parallel for num_threads(threads)
+  for (int64_t i = 0; i < n; ++i) {
+    const float* zi = z + i * V;
+    const RowSum r = row_sum(zi, V, inv_t);
+    const double o = origin(r.m), logz = r.z == 0 ? 0.0 : std::log(r.z);
+    const int64_t t = tok[i];
+    stat[i] = t >= 0 && t < V ? (float)((zi[t] - o) * inv_t - logz) : (t == -1 ? 0.f : kNan);
+    stat[n + i] = r.z == 0 ? 0.f : (float)(logz - r.u / r.z);
+    stat[2 * n + i] = (float)r.m;
+    stat[3 * n + i] = (float)r.z;
+    if (k > 0) {
+      int32_t* idx = scratch.mine();
+      std::iota(idx, idx + V, 0);
+      std::partial_sort(idx, idx + k, idx + V, [&](int32_t a, int32_t b) { return before(zi, a, b); });
+      for (int j = 0; j < k; ++j) {
+        top_col[i * k + j] = idx[j];
+        top_val[i * k + j] = (float)((zi[idx[j]] - o) * inv_t - logz);
       }
     }
   }
@@ -154,50 +175,50 @@ SPMM_HOST_EXPORT int spmm_cpu_token_logprobs_grad(int64_t n, int64_t V, const fl
 SPMM_HOST_EXPORT int spmm_cpu_distill(int64_t n, int64_t V, const float* z, const int64_t* rowptr, const int32_t* col,
                                       const float* val, int64_t nnz, double inv_t, float* loss, float* stat,
                                       const float* weight, float* out, int nthreads) {
-#pragma omp parallel num_threads(threads_or_default(nthreads))
-  {
-    std::vector<double> p((size_t)(out ? V : 0));
-#pragma omp for
-    for (int64_t i = 0; i < n; ++i) {
-      const float* zi = z + i * V;
-      const int64_t b = std::min(std::max<int64_t>(rowptr[i], 0), nnz);
-      const int64_t e = std::min(std::max(rowptr[i + 1], b), nnz);
-      double tm = kNoMass, ts = 0;
-      bool bad = false;
-      for (int64_t k = b; k < e; ++k) {
-        bad |= col[k] < -1 || col[k] >= V;
-        if (col[k] != -1 && val[k] > tm) tm = val[k];
-      }
-      const double to = origin(tm);
-      for (int64_t k = b; k < e; ++k)
-        if (col[k] != -1) ts += std::exp((val[k] - to) * inv_t);
-      bad |= ts != ts;
-      const RowSum r = row_sum(zi, V, inv_t);
-      const double o = origin(r.m), logz = r.z == 0 ? 0.0 : std::log(r.z);
-      double l = 0;
-      if (out) std::fill(p.begin(), p.end(), 0.0);
-      if (ts != 0 && !bad)
-        for (int64_t k = b; k < e; ++k) {
-          if (col[k] == -1) continue;
-          const double u = (val[k] - to) * inv_t, pk = std::exp(u) / ts;
-          if (pk != 0) l += pk * ((u - std::log(ts)) - ((zi[col[k]] - o) * inv_t - logz));
-          if (out) p[(size_t)col[k]] += pk;
-        }
-      loss[i] = bad ? kNan : (float)l;
-      stat[4 * i] = (float)r.m;
-      stat[4 * i + 1] = bad ? kNan : (float)r.z;
-      stat[4 * i + 2] = (float)to;
-      stat[4 * i + 3] = bad ? kNan : (float)ts;
-      if (!out) continue;
-      const double w = (weight ? weight[i] : 1.0) * inv_t;
-      float* oi = out + i * V;
-      if (w == 0 || (ts == 0 && !bad)) {
-        std::fill(oi, oi + V, 0.f);
-        continue;
-      }
-      for (int64_t j = 0; j < V; ++j)
-        oi[j] = bad ? kNan : (float)(w * ((r.z == 0 ? 0.0 : std::exp((zi[j] - o) * inv_t) / r.z) - p[(size_t)j]));
+  const int threads = threads_or_default(nthreads);
+  Scratch<double> scratch;
+  if (!scratch.make(threads, out ? V : 0)) return ENOMEM;
+#pragma omp parallel for num_threads(threads)
+  for (int64_t i = 0; i < n; ++i) {
+    double* p = scratch.mine();
+    const float* zi = z + i * V;
+    const int64_t b = std::min(std::max<int64_t>(rowptr[i], 0), nnz);
+    const int64_t e = std::min(std::max(rowptr[i + 1], b), nnz);
+    double tm = kNoMass, ts = 0;
+    bool bad = false;
+    for (int64_t k = b; k < e; ++k) {
+      bad |= col[k] < -1 || col[k] >= V;
+      if (col[k] != -1 && val[k] > tm) tm = val[k];
     }
+    const double to = origin(tm);
+    for (int64_t k = b; k < e; ++k)
+      if (col[k] != -1) ts += std::exp((val[k] - to) * inv_t);
+    bad |= ts != ts;
+    const RowSum r = row_sum(zi, V, inv_t);
+    const double o = origin(r.m), logz = r.z == 0 ? 0.0 : std::log(r.z);
+    double l = 0;
+    if (out) std::fill(p, p + V, 0.0);
+    if (ts != 0 && !bad)
+      for (int64_t k = b; k < e; ++k) {
+        if (col[k] == -1) continue;
+        const double u = (val[k] - to) * inv_t, pk = std::exp(u) / ts;
+        if (pk != 0) l += pk * ((u - std::log(ts)) - ((zi[col[k]] - o) * inv_t - logz));
+        if (out) p[col[k]] += pk;
+      }
+    loss[i] = bad ? kNan : (float)l;
+    stat[4 * i] = (float)r.m;
+    stat[4 * i + 1] = bad ? kNan : (float)r.z;
+    stat[4 * i + 2] = (float)to;
+    stat[4 * i + 3] = bad ? kNan : (float)ts;
+    if (!out) continue;
+    const double w = (weight ? weight[i] : 1.0) * inv_t;
+    float* oi = out + i * V;
+    if (w == 0 || (ts == 0 && !bad)) {
+      std::fill(oi, oi + V, 0.f);
+      continue;
+    }
+    for (int64_t j = 0; j < V; ++j)
+      oi[j] = bad ? kNan : (float)(w * ((r.z == 0 ? 0.0 : std::exp((zi[j] - o) * inv_t) / r.z) - p[j]));
   }
   return 0;
 }
