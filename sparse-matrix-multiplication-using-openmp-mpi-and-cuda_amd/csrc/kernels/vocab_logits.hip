@@ -555,7 +555,8 @@ __global__ __launch_bounds__(kThreads) void vocab_token_grad(TokenGradArgs a) {
 #pragma unroll
       for (int i = 0; i < n_; ++i) {
         const float u = (x[i] - o) * a.c, e = __builtin_amdgcn_exp2f(u);
-        x[i] = ENT ? e * __builtin_fmaf(beta, fmaxf(u, -1e30f), alpha) : e * alpha;   // (0 times -inf)
+        // (e is 0 from -150 down; beta u stays finite for every beta up to 3e34)
+        x[i] = ENT ? e * __builtin_fmaf(beta, fmaxf(u, -1e4f), alpha) : e * alpha;
       }
       const int64_t at = id - col;
       if (at >= 0 && at < n_) {
@@ -685,8 +686,18 @@ __global__ __launch_bounds__(kThreads) void distill_grad(DistillArgs a) {
 // A wave a row.  LOSS: the loss and the row's statistics.  With an output, what
 // distill_grad left at the teacher's entries is replaced by w (q - p) / T, the
 // p of equal columns summed in their order, rounded once.
+constexpr int kPlaceBits = 13, kRange = 32768;
+union FinishLds {   // of one wave
+  uint8_t place[1 << kPlaceBits];
+  struct {
+    uint32_t seen[kRange / 32], twice[kRange / 32];
+  } bits;
+};
+
 template <typename T, bool LOSS>
 __global__ __launch_bounds__(kThreads) void distill_finish(DistillArgs a) {
+  __shared__ FinishLds lds[kThreads / 64];
+  FinishLds& s = lds[threadIdx.x >> 6];
   const int lane = threadIdx.x & 63;
   for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.n; row += (int64_t)gridDim.x * 4) {
     // what does not depend on the row pointer is on its way while that is read
@@ -703,6 +714,9 @@ __global__ __launch_bounds__(kThreads) void distill_finish(DistillArgs a) {
       val = first ? val0 : i < e ? a.t.at(i) : 0.f;
     };
     const float l2t = log2_of(ts);
+    auto share_of = [&](int32_t col, float val) {
+      return col != -1 ? __builtin_amdgcn_exp2f((val - tm) * a.c - l2t) : 0.f;
+    };
     RowStat st;
     if (LOSS) {
       st = join_parts(a.part + row * a.S, a.S, a.c);
@@ -729,25 +743,76 @@ __global__ __launch_bounds__(kThreads) void distill_finish(DistillArgs a) {
     if (!a.out || wt == 0.f || ts == 0.f) continue;
     const float o = origin(st.m), scale = st.z == 0.f ? 0.f : wt / st.z;
     T* out = static_cast<T*>(a.out) + row * a.ldo;
-    for (int64_t base = b; base < e; base += 64) {
-      const int64_t i = base + lane;
-      int32_t mine, col;
-      float val;
-      entry(i, mine, val);
-      bool first = mine >= 0 && mine < a.V;
-      float p = 0.f;
+    auto write = [&](int32_t col, float x, float p) {
+      out[col] = Elem<T>::cast(exp2_of(x, o, a.c) * scale - wt * p);
+    };
+    // the p of the row's entries whose column is a lane's, in order, and whether entry i, that lane's, is the first
+    auto search = [&](int64_t i, int32_t mine, float& p, bool& first) {
+      p = 0.f;
       for (int64_t from = b; from < e; from += 64) {
+        int32_t col;
+        float val;
         entry(from + lane, col, val);
-        const float share = col != -1 ? __builtin_amdgcn_exp2f((val - tm) * a.c - l2t) : 0.f;
-        const int count = (int)(e - from < 64 ? e - from : 64);
+        const float share = share_of(col, val);
+        const int count = (int)(e - from < 64 ? e - from : 64), before = (int)(i - from < 64 ? i - from : 64);
         for (int j = 0; j < count; ++j) {
           const bool same = (int32_t)__builtin_amdgcn_readlane((uint32_t)col, j) == mine;
-          first = first && !(same && from + j < i);
           const float share_j = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(share), j));
           p += same ? share_j : 0.f;
+          first = first && !(same && j < before);
         }
       }
-      if (first) out[mine] = Elem<T>::cast(exp2_of(base == b ? x0 : a.picked[i], o, a.c) * scale - wt * p);
+    };
+    if (e - b <= 64) {
+      // Equal columns meet in a table: the lane that is left in a place is done, one that finds its own column
+      // there has an equal, one that finds another's goes on (two rounds mostly; the search costs 5 us).
+      const bool mine = col0 >= 0 && col0 < a.V;
+      const uint32_t place = ((uint32_t)col0 * 0x9e3779b1u) >> (32 - kPlaceBits);
+      bool open = mine, equal = false;
+      while (__ballot(open) != 0 && __ballot(equal) == 0) {
+        if (open) s.place[place] = (uint8_t)lane;
+        wave_fence();
+        const int left = open ? (int)s.place[place] : lane;
+        wave_fence();
+        equal = __shfl(col0, left) == col0 && left != lane;
+        open = open && left != lane;
+      }
+      float p = share_of(col0, val0);
+      bool first = mine;
+      if (__ballot(equal) != 0) search(b + lane, col0, p, first);
+      if (first) write(col0, x0, p);
+      continue;
+    }
+    // More entries: a range of columns at a time, in one bit a column, or, where a few entries stand against many
+    // ranges, by searching for all of them.
+    const int64_t chunks = (e - b + 63) / 64, ranges = (a.V + kRange - 1) / kRange;
+    const bool by_range = ranges * (chunks + 3) <= 10 * chunks * chunks;
+    for (int64_t r = 0; r < (by_range ? ranges : 1); ++r) {
+      const int64_t lo = r * kRange, hi = by_range && lo + kRange < a.V ? lo + kRange : a.V;
+      if (by_range) {
+        for (int i = lane; i < kRange / 32; i += 64) s.bits.seen[i] = s.bits.twice[i] = 0u;
+        wave_fence();
+        for (int64_t i = b + lane; i < e; i += 64) {
+          const int32_t col = a.t.col[i];
+          if (col < lo || col >= hi) continue;
+          const int at = (int)(col - lo) >> 5;
+          const uint32_t bit = 1u << (col & 31);
+          if (atomicOr(&s.bits.seen[at], bit) & bit) atomicOr(&s.bits.twice[at], bit);
+        }
+        wave_fence();
+      }
+      for (int64_t base = b; base < e; base += 64) {
+        int32_t col;
+        float val;
+        entry(base + lane, col, val);
+        const bool mine = col >= lo && col < hi;
+        const bool equal = !by_range || (mine && ((s.bits.twice[(int)(col - lo) >> 5] >> (col & 31)) & 1));
+        float p = share_of(col, val);
+        bool first = mine;
+        if (__ballot(equal) != 0) search(base + lane, col, p, first);
+        if (first) write(col, a.picked[base + lane], p);
+      }
+      wave_fence();
     }
   }
 }

@@ -179,6 +179,19 @@ def test_grad_table_sizes(V):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [1, 4, 7])
+def test_grad_narrow_rows_of_a_frequent_token(dev, dtype, D):
+    g = gen(D)
+    V, n = 37, 50001
+    tok = torch.randint(-1, V + 1, (n,), generator=g)
+    tok[torch.rand(n, generator=g) < 0.8] = 5
+    dY = torch.randn(n, D, generator=g).to(dtype)
+    check_grad(dY, tok, V, 0.5, dtype, False, dev)
+    check_grad(dY, tok % 30, V, 0.5, torch.float32, True, dev)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_grad_layouts(dev):
     g = gen(2)
     V, D = 30, 20
@@ -318,6 +331,42 @@ def test_logprobs_long_rows_of_ties_and_infinities(dev, dtype):
         check_logprobs(z, tok, k, 1.0, dev)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_logprobs_rows_of_millions(dtype):
+    """More groups in a row than a wave keeps in registers."""
+    V = 9_000_001
+    z, tok = logits(2, V, dtype, seed=33)
+    z[1, ::3] = 4.5
+    for k in (2, 128):
+        check_logprobs(z, tok, k, 1.0, "cuda")
+
+
+@pytest.mark.gpu
+def test_more_rows_than_workgroups():
+    """Beyond the largest grid the workgroups go on with further rows: those have the results of a call of their own."""
+    n, V, last = (1 << 23) + 777, 9, 1000
+    z = torch.randn(n, V, generator=gen(34)).to(torch.bfloat16).cuda()
+    tok = torch.randint(0, V, (n,), generator=gen(35)).cuda()
+    g = torch.rand(n, generator=gen(36)).cuda()
+    a, b = token_logprobs(z, tok, k=3), token_logprobs(z[-last:], tok[-last:], k=3)
+    assert torch.equal(a.stat[:, -last:], b.stat)
+    assert torch.equal(a.top.col[-3 * last:], b.top.col) and torch.equal(a.top.val[-3 * last:], b.top.val)
+    dz = token_logprobs_grad(z, tok, a, g, g)
+    assert torch.equal(dz[-last:], token_logprobs_grad(z[-last:], tok[-last:], b, g[-last:], g[-last:]))
+    (la, da), (lb, db) = distill_loss_grad(z, a.top, g), distill_loss_grad(z[-last:], b.top, g[-last:])
+    assert torch.equal(la.loss[-last:], lb.loss) and torch.equal(da[-last:], db)
+    W = torch.randn(300, 520, generator=gen(37)).to(torch.bfloat16).cuda()
+    y = embedding(W, tok)
+    assert torch.equal(y[-last:], W[tok[-last:]])
+    few = torch.randint(0, 1 << 27, (500,), generator=gen(38)).cuda()
+    few[0] = (1 << 27) + 999
+    dW, used = embedding_grad(y[:500, :8], few, (1 << 27) + 1000), few.unique()
+    assert torch.equal(dW[used], embedding_grad(y[:500, :8], torch.searchsorted(used, few), used.numel()))
+    dW[used] = 0
+    assert torch.equal(dW, torch.zeros_like(dW))
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [3, 700, 20001])
@@ -400,6 +449,19 @@ def test_logprobs_grad_masks(dev):
     h[4] = 0.0                       # a padded row of garbage: nothing flows, nothing is read
     got = check_token_grad(z, tok, g, h, 1.5, dev)
     assert (got[4] == 0).all() and got[6].isnan().all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("T", [1e-12, 1e12])
+def test_logprobs_grad_temperatures(dev, T):
+    """Temperatures that leave the largest logit alone, or all of them alike."""
+    z, tok = logits(6, 700, torch.float32, seed=26)
+    z[1, 5:] = -math.inf
+    z[2, :300] = torch.finfo(torch.float32).min
+    z[3] = 0.25
+    tok[1] = 2
+    check_token_grad(z, tok, None, torch.randn(6, generator=gen(27)), T, dev)
+    check_token_grad(z, tok, torch.randn(6, generator=gen(28)), torch.randn(6, generator=gen(29)), T, dev)
 
 
 @pytest.mark.parametrize("dev", DEVICES)
@@ -506,6 +568,28 @@ def test_distill_many_rows(dtype, n, V):
     T = random_teacher(n, V, 40, seed=V)
     check_distill(z, T, 1.5, w, "cuda")
     check_distill(z, T, 1.0, w, "cuda", inplace=True)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_distill_long_teacher_rows(dev):
+    """Thousands of entries a row: ascending columns, absent ones behind them, one column twice, any order."""
+    V, L = 9000, 3001
+    z, _ = logits(5, V, torch.float32, seed=30)
+    g = gen(31)
+    rows = []
+    for i in range(5):
+        c = torch.randperm(V, generator=g)[:L]
+        c = c if i == 4 else c.sort().values
+        if i == 1:
+            c[2000:] = -1
+        if i == 2:
+            c[1500] = c[1499]
+        if i == 3:
+            c[10] = -1                                     # absent in the middle
+        rows.append([(int(x), float(v)) for x, v in zip(c, torch.randn(L, generator=g) * 2)])
+    w = torch.rand(5, generator=gen(32)) + 0.1
+    for dtype in (torch.float32, torch.bfloat16):
+        check_distill(z.to(dtype), teacher_of(rows, V), 1.5, w, dev, inplace=True)
 
 
 @pytest.mark.parametrize("dev", DEVICES)
