@@ -265,9 +265,9 @@ __device__ __forceinline__ int wave_scan(int x) {
 //
 // `from`, a key that at least k elements reach, starts as the k-th largest of
 // the groups' maxima.  The elements that reach it are collected from the groups
-// whose maxima do.  More than kCand: the k-th largest of those in hand is a
-// better bound, or, if it is the same one, only elements above it are
-// collected, and of its equals the lowest columns are looked up in the row.
+// whose maxima do.  More than kCand: the k-th largest of a sample is a better
+// bound, or, if it is the same one, only elements above it are collected, and
+// of its equals the lowest columns are looked up in the row.
 //
 // A wave runs this once, alone on its SIMD or nearly so, and its time goes into
 // round trips to memory and into fetching code that no wave has run before: the
@@ -350,7 +350,9 @@ __device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& 
       const unsigned long long m = __ballot(in && reaches(x));
       if (m == 0) return;
       const int at = count + __popcll(m & below);
-      if (((m >> lane) & 1) && at < kCand) s.cand[at] = entry_of(key_of(x), col);
+      // (of more than kCand a sample of all, so that the next bound leaves a quarter whatever their order)
+      const uint32_t slot = at < kCand ? (uint32_t)at : __umulhi((uint32_t)at * 0x9e3779b1u, (uint32_t)at + 1u);
+      if (((m >> lane) & 1) && slot < kCand) s.cand[slot] = entry_of(key_of(x), col);
       count += __popcll(m);
     };
     const int vecs = z.nv > 0 ? hits << slots_log : 0;   // (a short row may have extra elements alone)
