@@ -238,14 +238,16 @@ struct JoinArgs {
   float* top_val;
 };
 
-constexpr int kCand = 512;      // candidates of a row that are ranked against each other
+constexpr int kCand = 448;      // candidates of a row that are ranked against each other
 constexpr int kHits = 256;      // groups of a row that are read again
 constexpr int kKeyRegs = 16;    // groups of a row whose maxima a lane keeps
 constexpr int kFlight = 4;      // vectors of a lane that are read at a time
 
-struct TopLds {   // of one wave
+struct TopLds {   // of one wave (four workgroups a CU)
   uint64_t cand[kCand + 8];
   int hit[kHits];
+  u32x4 vec[64 * kFlight];   // vectors with a candidate
+  int at[64 * kFlight];
 };
 
 __device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
@@ -300,20 +302,37 @@ __device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& 
     }
   };
 
-  // the k-th largest key, bit by bit; reach(key): how many are not below it
-  auto kth_largest = [&](auto&& reach) {
-    uint32_t key = 0;
+  // a key that at least k reach, the k-th largest of them unless exactly k do, between lo and hi bit by bit;
+  // reach(key): how many are not below it
+  auto kth_largest = [&](uint32_t lo, uint32_t hi, auto&& reach) {
+    uint32_t key = hi;
+    int b = lo == hi ? -1 : 31 - __builtin_clz(lo ^ hi);
+    if (b >= 0) key &= ~1u << b;
 #pragma unroll 1
-    for (int b = 31; b >= Elem<T>::kLowBits; --b) {
+    for (; b >= Elem<T>::kLowBits; --b) {
       const uint32_t trial = key | (1u << b);
-      if (reach(trial) >= k) key = trial;
+      const int c = reach(trial);
+      if (c >= k) key = trial;
+      if (c == k) break;
     }
     // the bits that the type does not have: ones in negative keys and in NaN's
     if (!(key & 0x80000000u) || key > key_of(kInf)) key |= (1u << Elem<T>::kLowBits) - 1u;
     return key;
   };
+  // the lanes' largest key, or second largest, is reached by 64 or 128 keys
+  uint32_t first = 0, second = 0;
+  if (in_regs) {
+#pragma unroll
+    for (int j = 0; j < kKeyRegs; ++j) {
+      const uint32_t low = first < held[j] ? first : held[j];
+      second = max_u(second, low);
+      first = max_u(first, held[j]);
+    }
+  }
+  const uint32_t least = over_wave(k <= 64 ? first : second, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+  const uint32_t most = in_regs ? over_wave(first, max_u) : ~0u;
   // (64 bits: it may pass the largest key)
-  uint64_t from = kth_largest([&](uint32_t trial) {
+  uint64_t from = kth_largest(least, most, [&](uint32_t trial) {
     int c = 0;
     each_key([&](int, uint32_t key) { c += __popcll(__ballot(key >= trial)); });
     return c;
@@ -346,6 +365,7 @@ __device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& 
     const bool only_nan = from > key_of(kInf);
     const float bound = only_nan ? 0.f : value_of((uint32_t)from);
     auto reaches = [&](float x) { return only_nan ? x != x && from <= 0xffffffffu : !(x < bound); };
+    const float may = only_nan ? kInf : bound;   // what reaches `from` is not below it
     auto offer = [&](bool in, float x, int col) {   // (most lanes have nothing)
       const unsigned long long m = __ballot(in && reaches(x));
       if (m == 0) return;
@@ -372,12 +392,28 @@ __device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& 
         v[f] = place(i0 + f * 64 + lane);
         x[f] = z.vec(v[f] < 0 ? 0 : v[f]);
       }
+      int many = 0;
 #pragma unroll
       for (int f = 0; f < kFlight; ++f) {
-        if (i0 + f * 64 >= vecs) break;
+        bool any = false;
 #pragma unroll
-        for (int e = 0; e < N; ++e) offer(v[f] >= 0, Elem<T>::get(x[f], e), z.col(v[f]) + e);
+        for (int e = 0; e < N; ++e) any |= !(Elem<T>::get(x[f], e) < may);
+        const unsigned long long m = __ballot(any && v[f] >= 0);
+        const int at = many + __popcll(m & below);
+        if ((m >> lane) & 1) {
+          s.vec[at] = x[f];
+          s.at[at] = v[f];
+        }
+        many += __popcll(m);
       }
+      wave_fence();
+#pragma unroll 1
+      for (int i = lane; i - lane < many * N; i += 64) {
+        const bool in = i < many * N;
+        const int h = in ? i / N : 0;
+        offer(in, Elem<T>::load(reinterpret_cast<const T*>(s.vec + h) + i % N), z.col(s.at[h]) + i % N);
+      }
+      wave_fence();
     }
     {
       const int c = z.extra(lane);
@@ -385,7 +421,7 @@ __device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& 
     }
     wave_fence();
     if (count <= kCand) break;
-    const uint32_t better = kth_largest([&](uint32_t trial) {
+    const uint32_t better = kth_largest(0u, ~0u, [&](uint32_t trial) {
       int c = 0;
 #pragma unroll 1
       for (int i = 0; i < kCand; i += 64) c += __popcll(__ballot((uint32_t)(s.cand[i + lane] >> 32) >= trial));
