@@ -12,6 +12,7 @@
 //          second kernel adds in tile order: a token that fills a tenth of the
 //          batch costs the same as any other.  Rows without a token are written
 //          as zeros by further workgroups of the same launch, or of the sort's.
+//          A short batch is not sorted at all (embed_grad_brief).
 #include "vocab_common.hpp"
 
 using namespace spmm;
@@ -82,6 +83,17 @@ int lookup(const T* W, int64_t ldw, int64_t V, int64_t D, const void* tok, int w
   return 0;
 }
 
+// `bytes` zeros from thread `first` of `threads` on: vectors, then the last columns
+__device__ __forceinline__ void zero_table(uint16_t* table, int64_t bytes, int64_t first, int64_t threads) {
+  const int64_t vecs = bytes / 16;
+  for (int64_t i = first; i < vecs; i += threads) store_vec(table + i * 8, u32x4{0u, 0u, 0u, 0u});
+  if (first < (bytes & 15) / 2) table[vecs * 8 + first] = 0;
+}
+
+__global__ __launch_bounds__(256) void embed_zero(uint16_t* __restrict__ table, int64_t bytes) {
+  zero_table(table, bytes, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+}
+
 // ---- sort of (token, position) ------------------------------------------------
 // Keys: the token, or V for padding and for tokens outside the table (sorted
 // last, summed nowhere).  The last pass also writes slot[token], one of the
@@ -104,8 +116,7 @@ constexpr int kRankWaves = 16;
 // A table of which the batch has few rows, without gaps between them, is zeroed
 // by further workgroups of this launch (`bytes` of it), before any row is
 // known: the sort hides behind that.  8000 tokens over 65536 x 4096 bf16: 120 us
-// instead of 133, 12000 over 131072 x 513: 55 instead of 63; one token over 1
-// GiB, where there is nothing to hide: 176 instead of 172.
+// instead of 133, 12000 over 131072 x 513: 55 instead of 63.
 constexpr int64_t kFewRows = 8;   // table rows for each token, from which on
 
 __global__ __launch_bounds__(64 * kRankWaves) void embed_rank_sort(const void* __restrict__ tok, int wide, int n,
@@ -117,10 +128,8 @@ __global__ __launch_bounds__(64 * kRankWaves) void embed_rank_sort(const void* _
   __shared__ int part[kRankWaves][64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, sorts = (n + 63) / 64;
   if ((int)blockIdx.x >= sorts) {
-    const int64_t vecs = bytes / 16, first = (int64_t)(blockIdx.x - sorts) * (64 * kRankWaves) + tid;
-    for (int64_t i = first; i < vecs; i += (int64_t)(gridDim.x - sorts) * (64 * kRankWaves))
-      store_vec(table + i * 8, u32x4{0u, 0u, 0u, 0u});
-    if (first < (bytes & 15) / 2) table[vecs * 8 + first] = 0;
+    zero_table(table, bytes, (int64_t)(blockIdx.x - sorts) * (64 * kRankWaves) + tid,
+               (int64_t)(gridDim.x - sorts) * (64 * kRankWaves));
     return;
   }
   const int i = blockIdx.x * 64 + lane;
@@ -358,6 +367,7 @@ struct GradArgs {
   void* dw;
   float* part;   // [tiles][2][D]: a tile's sums of the run it begins inside and of the one it ends inside
   int accumulate, zeroed;   // rows without a token: they keep their values; they are zero already
+  int brief;                // embed_grad_brief, without sorted entries
 };
 
 // Sorted entries a wave sums: 8 in a short batch, which has few waves to hide
@@ -644,6 +654,93 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_grad_join(GradArgs a) {
   }
 }
 
+// Few tokens: a workgroup for each token and slice of columns looks for its
+// token among all of them and, if it is the first such place, sums the rows in
+// order: no sort, one launch, and one before it that zeroes the table.  1000
+// tokens over 8192 x 1024 bf16: 10.3 us (sorted: 16.1), added to an fp32 table
+// 6.3 (15.2); 777 of mixed frequency over 32003 x 1000 16.1 (22.3).  One token
+// only, which no batch is: 777 times 49 (24.5).
+constexpr int kBriefTokens = 1024;
+constexpr int64_t kBriefGroups = 4096;   // two rounds of the chip
+constexpr int kBriefWaves = 8, kBriefFlight = 8;   // 4 waves: a run of 777 112 us; 16 rows in flight: 1000 x 1024 20
+
+template <typename TI, typename TO>
+__global__ __launch_bounds__(64 * kBriefWaves) void embed_grad_brief(GradArgs a, const void* __restrict__ tok,
+                                                                     int wide) {
+  constexpr int N = Elem<TI>::kN, kRounds = kBriefTokens / (64 * kBriefWaves);
+  __shared__ int list[kBriefTokens];
+  __shared__ int found[kBriefWaves];
+  __shared__ float sums[kBriefWaves - 1][64 * N];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = (int)a.n, slices = (int)a.slices;
+  const int i = (int)blockIdx.x / slices;
+  const int64_t c = ((int64_t)((int)blockIdx.x - i * slices) * 64 + lane) * N, from = c + N <= a.D ? c : a.D - N;
+  const int64_t key = token_at(tok, wide, i);
+  int64_t t[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int p = (w * kRounds + r) * 64 + lane;
+    t[r] = token_at(tok, wide, p < n ? p : n - 1);
+  }
+  if (key < 0 || key >= a.V) return;
+  unsigned long long same[kRounds];
+  int count = 0;
+  bool later = false;   // an earlier token is the same
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int p = (w * kRounds + r) * 64 + lane;
+    same[r] = __ballot(p < n && t[r] == key);
+    later = later || __ballot(p < i && t[r] == key) != 0;
+    count += __popcll(same[r]);
+  }
+  if (lane == 0) found[w] = later ? -kBriefTokens : count;
+  __syncthreads();
+  int total = 0, at = 0;
+#pragma unroll
+  for (int q = 0; q < kBriefWaves; ++q) {
+    at = q == w ? total : at;
+    total += found[q];
+  }
+  if (total <= 0) return;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    if ((same[r] >> lane) & 1) list[at + __popcll(same[r] & ((1ull << lane) - 1ull))] = (w * kRounds + r) * 64 + lane;
+    at += __popcll(same[r]);
+  }
+  __syncthreads();
+  const bool shared = total > kBriefFlight;   // (by the waves)
+  const int first = shared ? total * w / kBriefWaves : 0;
+  const int last = shared ? total * (w + 1) / kBriefWaves : w == 0 ? total : 0;
+  float acc[N] = {};
+  for (int q = first; q < last; q += kBriefFlight) {
+    Cols<TI, N> x[kBriefFlight];
+#pragma unroll
+    for (int u = 0; u < kBriefFlight; ++u) {
+      const int64_t row = __builtin_amdgcn_readfirstlane(list[q + u < last ? q + u : last - 1]);
+      x[u].load(static_cast<const TI*>(a.dy) + row * a.lddy, from);
+    }
+#pragma unroll
+    for (int u = 0; u < kBriefFlight; ++u) {
+      if (q + u >= last) break;
+#pragma unroll
+      for (int s = 0; s < N; ++s) acc[s] += x[u].get(s);
+    }
+  }
+  if (shared) {
+    if (w > 0) {
+#pragma unroll
+      for (int s = 0; s < N; ++s) sums[w - 1][s * 64 + lane] = acc[s];
+    }
+    __syncthreads();
+    if (w == 0) {
+#pragma unroll
+      for (int q = 0; q < kBriefWaves - 1; ++q)
+#pragma unroll
+        for (int s = 0; s < N; ++s) acc[s] += sums[q][s * 64 + lane];
+    }
+  }
+  if (w == 0 && c < a.D) finish_row<TO, N>(a, key, c, from, acc);
+}
+
 struct GradSizes {
   int64_t tile, tiles, sort_tiles, keys, cnt, slots, total;
   int bits, passes, rounds;
@@ -670,7 +767,18 @@ bool grad_sizes(int64_t n, int64_t V, int64_t D, GradSizes& g) {
 }
 
 template <typename TI, typename TO>
-int grad(GradArgs a, hipStream_t s) {
+int grad(GradArgs a, const void* tok, int wide, hipStream_t s) {
+  if (a.brief) {
+    const int64_t bytes = a.V * a.D * (int64_t)sizeof(TO);
+    if (!a.accumulate)
+      hipLaunchKernelGGL(embed_zero, dim3(groups_of((bytes + 4095) / 4096)), dim3(256), 0, s,
+                         static_cast<uint16_t*>(a.dw), bytes);
+    if (a.n > 0)
+      hipLaunchKernelGGL((embed_grad_brief<TI, TO>), dim3((unsigned)(a.n * a.slices)),
+                         dim3(64 * kBriefWaves), 0, s, a, tok, wide);
+    SPMM_LAUNCH_CHECK();
+    return 0;
+  }
   if (a.D < kNarrow) {
     hipLaunchKernelGGL((embed_grad_narrow<TI, TO>), dim3(groups_of((a.V + 3) / 4)), dim3(256), 0, s, a);
     SPMM_LAUNCH_CHECK();
@@ -722,7 +830,12 @@ SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, c
   int32_t* slot = accumulate ? nullptr : pa + g.keys;
   char* behind = reinterpret_cast<char*>(pa + g.keys + g.slots);
   int64_t zeroed = 0;   // bytes of the table that the sort's launch zeroes
-  if (n > kRankMax) {
+  const int lane_cols = in_type == kF32 ? 4 : 8;
+  const int64_t slices = (D + 64 * lane_cols - 1) / (64 * lane_cols);
+  const bool brief = n <= kBriefTokens && n * slices <= kBriefGroups && D >= kNarrow && (accumulate || ldw == D);
+  if (brief) {
+    // no sort
+  } else if (n > kRankMax) {
     uint32_t* kb = reinterpret_cast<uint32_t*>(behind);
     int32_t* pb = reinterpret_cast<int32_t*>(kb + g.keys);
     int32_t* cnt = pb + g.keys;
@@ -773,10 +886,11 @@ SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, c
   a.part = reinterpret_cast<float*>(behind);
   a.accumulate = accumulate;
   a.zeroed = zeroed != 0;
+  a.slices = slices;
+  a.brief = brief;
   SPMM_VOCAB_TYPE(in_type, TI, {
-    a.slices = (D + 64 * Elem<TI>::kN - 1) / (64 * Elem<TI>::kN);
-    if (out_type == kF32) return grad<TI, float>(a, s);
-    if (out_type == in_type) return grad<TI, TI>(a, s);
+    if (out_type == kF32) return grad<TI, float>(a, tok, wide, s);
+    if (out_type == in_type) return grad<TI, TI>(a, tok, wide, s);
     return (int)hipErrorInvalidValue;
   });
   return 0;

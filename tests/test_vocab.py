@@ -180,6 +180,27 @@ def test_grad_table_sizes(V):
 
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,D", [(1, 9, 8), (8, 5, 513), (9, 70, 64), (64, 2, 1000), (65, 4000, 33), (300, 1, 40),
+                                   (1000, 100, 4100), (1024, 333, 72), (1025, 333, 72), (0, 40, 9)])
+def test_grad_short_batches(dev, dtype, n, V, D):
+    """Batches on both sides of what is summed without a sort, into tables with and without gaps between the rows."""
+    g = gen(n + D)
+    tok = torch.randint(-1, V + 1, (n,), generator=g)
+    tok[: n // 3] = V - 1
+    dY = torch.randn(n, D, generator=g).to(dtype)
+    ref, mag, count = ref_grad(dY, tok, V, 1.25)
+    tol = half_step(dtype, ref) + (count + 4) * U * mag
+    for wide in (D, D + 24):
+        table = torch.full((V + 1, wide), 7.0, dtype=dtype, device=dev)
+        out = table[:V, :D]
+        assert embedding_grad(dY.to(dev), tok.to(dev), V, scale=1.25, out=out) is out
+        near(out, ref, tol)
+        assert (table[V] == 7).all() and (table[:, D:] == 7).all()
+    check_grad(dY, tok.to(torch.int32), V, 1.25, torch.float32, True, dev)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("D", [1, 4, 7])
 def test_grad_narrow_rows_of_a_frequent_token(dev, dtype, D):
     g = gen(D)
