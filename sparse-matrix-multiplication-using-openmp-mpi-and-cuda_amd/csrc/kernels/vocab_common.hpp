@@ -2,8 +2,9 @@
 //
 // Dense rows are fp32, bf16 or fp16, any row stride, any base alignment that
 // the element type has: 16-byte loads and stores are typed with the element's
-// own alignment (gfx950 takes unaligned global accesses), so a vocabulary of
-// odd size costs one more cache line a wave and no peeled head.
+// own alignment, which gfx950 takes.  They cost a quarter of the bandwidth where
+// they are not aligned: long rows start at the next 16-byte boundary instead
+// (vocab_logits.hip Row).
 #pragma once
 #include "common.hpp"
 
