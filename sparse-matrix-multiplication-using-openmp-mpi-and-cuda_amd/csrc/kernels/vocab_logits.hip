@@ -55,6 +55,10 @@ struct Row {
     return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(z + head + (int64_t)v * N));
   }
   __device__ __forceinline__ int col(int v) const { return head + v * N; }
+  // the vector that holds a column, -1: an extra element does
+  __device__ __forceinline__ int vec_of(int c) const {
+    return c < head || c >= head + nv * N ? -1 : (c - head) / N;
+  }
   // column of extra element x of 2 N, or -1
   __device__ __forceinline__ int extra(int x) const {
     const int c = x < N ? (x < head ? x : -1) : head + nv * N + (x - N);
@@ -73,6 +77,11 @@ struct Walk {
   int step;       // 1 or 8
   __device__ __forceinline__ int page(int seg, int j, int vpt) const {
     return step == 1 ? seg * vpt + j : ((seg >> 3) * vpt + j) * 8 + (seg & 7);
+  }
+  // the workgroup that has a vector (-1: an extra element)
+  __device__ __forceinline__ int seg_of(int vec, int vpt) const {
+    const int p = vec / 256;
+    return vec < 0 ? 0 : step == 1 ? p / vpt : p / (8 * vpt) * 8 + (p & 7);
   }
 };
 
@@ -685,18 +694,152 @@ __global__ __launch_bounds__(kThreads) void distill_stats(StatsArgs s, DistillAr
   }
 }
 
+// A row's end, by one wave.  loss: the loss and the row's statistics.  With an
+// output, what distill_grad left at the teacher's entries of columns that
+// own(column) names is replaced by w (q - p) / T, the p of equal columns summed
+// in their order, rounded once.
+constexpr int kPlaceBits = 13, kRange = 32768;
+union FinishLds {   // of one wave
+  uint8_t place[1 << kPlaceBits];
+  struct {
+    uint32_t seen[kRange / 32], twice[kRange / 32];
+  } bits;
+};
+
+template <typename T, typename F>
+__device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, FinishLds& s, RowStat st, bool loss,
+                                           F&& own) {
+  const int lane = threadIdx.x & 63;
+  // what does not depend on the row pointer is on its way while that is read
+  const float tm = a.stat[row * 4 + 2], ts = a.stat[row * 4 + 3], wt = (a.weight ? a.weight[row] : 1.f) * a.inv_t;
+  int64_t b, e;
+  a.t.range(row, b, e);
+  // a lane's entry of the first 64 (most rows have no more) is read once
+  const bool has = b + lane < e;
+  const int32_t col0 = has ? a.t.col[b + lane] : -1;
+  const float val0 = has ? a.t.at(b + lane) : 0.f, x0 = has ? a.picked[b + lane] : 0.f;
+  auto entry = [&](int64_t i, int32_t& col, float& val) {
+    const bool first = i == b + lane;
+    col = first ? col0 : i < e ? a.t.col[i] : -1;
+    val = first ? val0 : i < e ? a.t.at(i) : 0.f;
+  };
+  const float l2t = log2_of(ts);
+  auto share_of = [&](int32_t col, float val) {
+    return col != -1 ? __builtin_amdgcn_exp2f((val - tm) * a.c - l2t) : 0.f;
+  };
+  if (loss) {
+    const float o = origin(st.m), l2z = log2_of(st.z);
+    float sum = 0.f;
+    for (int64_t i = b + lane; i < e; i += 64) {
+      int32_t col;
+      float val;
+      entry(i, col, val);
+      if (col < 0 || col >= a.V) continue;
+      const float u = (val - tm) * a.c - l2t, p = __builtin_amdgcn_exp2f(u), x = i == b + lane ? x0 : a.picked[i];
+      if (!(p == 0.f)) sum += p * (kLn2 * u - ((x - o) * a.inv_t - kLn2 * l2z));
+    }
+    sum = wave_sum(sum);
+    if (ts != ts) sum = st.z = ts;   // a column outside the vocabulary, or a NaN
+    if (lane == 0) {
+      a.loss[row] = ts == 0.f ? 0.f : sum;   // (no mass: nothing to learn)
+      a.stat[row * 4] = st.m;
+      a.stat[row * 4 + 1] = st.z;
+    }
+  }
+  if (!a.out || wt == 0.f || ts == 0.f) return;
+  const float o = origin(st.m), scale = st.z == 0.f ? 0.f : wt / st.z;
+  T* out = static_cast<T*>(a.out) + row * a.ldo;
+  auto write = [&](int32_t col, float x, float p) {
+    out[col] = Elem<T>::cast(exp2_of(x, o, a.c) * scale - wt * p);
+  };
+  // the p of the row's entries whose column is a lane's, in order, and whether entry i, that lane's, is the first
+  auto search = [&](int64_t i, int32_t mine, float& p, bool& first) {
+    p = 0.f;
+    for (int64_t from = b; from < e; from += 64) {
+      int32_t col;
+      float val;
+      entry(from + lane, col, val);
+      const float share = share_of(col, val);
+      const int count = (int)(e - from < 64 ? e - from : 64), before = (int)(i - from < 64 ? i - from : 64);
+      for (int j = 0; j < count; ++j) {
+        const bool same = (int32_t)__builtin_amdgcn_readlane((uint32_t)col, j) == mine;
+        const float share_j = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(share), j));
+        p += same ? share_j : 0.f;
+        first = first && !(same && j < before);
+      }
+    }
+  };
+  if (e - b <= 64) {
+    // Equal columns meet in a table: the lane that is left in a place is done, one that finds its own column
+    // there has an equal, one that finds another's goes on (two rounds mostly; the search costs 5 us).
+    const bool mine = col0 >= 0 && col0 < a.V && own(col0);
+    const uint32_t place = ((uint32_t)col0 * 0x9e3779b1u) >> (32 - kPlaceBits);
+    bool open = mine, equal = false;
+    while (__ballot(open) != 0 && __ballot(equal) == 0) {
+      if (open) s.place[place] = (uint8_t)lane;
+      wave_fence();
+      const int left = open ? (int)s.place[place] : lane;
+      wave_fence();
+      equal = __shfl(col0, left) == col0 && left != lane;
+      open = open && left != lane;
+    }
+    float p = share_of(col0, val0);
+    bool first = mine;
+    if (__ballot(equal) != 0) search(b + lane, col0, p, first);
+    if (first) write(col0, x0, p);
+    return;
+  }
+  // More entries: a range of columns at a time, in one bit a column, or, where a few entries stand against many
+  // ranges, by searching for all of them.
+  const int64_t chunks = (e - b + 63) / 64, ranges = (a.V + kRange - 1) / kRange;
+  const bool by_range = ranges * (chunks + 3) <= 10 * chunks * chunks;
+  for (int64_t r = 0; r < (by_range ? ranges : 1); ++r) {
+    const int64_t lo = r * kRange, hi = by_range && lo + kRange < a.V ? lo + kRange : a.V;
+    if (by_range) {
+      for (int i = lane; i < kRange / 32; i += 64) s.bits.seen[i] = s.bits.twice[i] = 0u;
+      wave_fence();
+      for (int64_t i = b + lane; i < e; i += 64) {
+        const int32_t col = a.t.col[i];
+        if (col < lo || col >= hi) continue;
+        const int at = (int)(col - lo) >> 5;
+        const uint32_t bit = 1u << (col & 31);
+        if (atomicOr(&s.bits.seen[at], bit) & bit) atomicOr(&s.bits.twice[at], bit);
+      }
+      wave_fence();
+    }
+    for (int64_t base = b; base < e; base += 64) {
+      int32_t col;
+      float val;
+      entry(base + lane, col, val);
+      const bool mine = col >= lo && col < hi && own(col);
+      const bool equal = !by_range || (mine && ((s.bits.twice[(int)(col - lo) >> 5] >> (col & 31)) & 1));
+      float p = share_of(col, val);
+      bool first = mine;
+      if (__ballot(equal) != 0) search(base + lane, col, p, first);
+      if (first) write(col, a.picked[base + lane], p);
+    }
+    wave_fence();
+  }
+}
+
 // w q / T everywhere.  JOIN: the rows' statistics are put together here, from
 // their segments'.
 //
 // Bytes bound a step of loss and gradient: the logits are read twice and the
-// gradient written once, 3.2 GB for 4096 x 131072 bf16 in 502 us (519 at the
+// gradient written once, 3.2 GB for 4096 x 131072 bf16 in 497 us (521 at the
 // rate of a large copy).  One read would take a row of 256 KB in registers
 // from its statistics to its gradient, half of a CU's: a workgroup a row with
 // half of it kept took 574 us, with all of it spilling 670, where these kernels
 // then took 580.  A second read out of the last-level cache (statistics and
 // gradient of 128 MB at a time) is no faster than one from memory: 660 us.
-template <typename T, int VPT, bool JOIN>
+//
+// FINISH: few workgroups, where a launch costs more than it does: each one ends
+// its own columns of the row itself, the first one the loss (48 x 32768 fp16, 32
+// entries: 8.4 us instead of 10.3, from the host 19.6 instead of 22.1; 1000 x
+// 32768, 8000 workgroups: 52.8 instead of 47.5).
+template <typename T, int VPT, bool JOIN, bool FINISH>
 __global__ __launch_bounds__(kThreads) void distill_grad(DistillArgs a) {
+  __shared__ std::conditional_t<FINISH, FinishLds, int> lds;
   const Walk wk = a.wk;
   const int64_t tasks = a.n * wk.S;
   for (int64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
@@ -705,8 +848,19 @@ __global__ __launch_bounds__(kThreads) void distill_grad(DistillArgs a) {
     const Row<T> z(a.z, a.ld, row, wk.V);
     T* out = static_cast<T*>(a.out) + row * a.ldo;
     const float wt = (a.weight ? a.weight[row] : 1.f) * a.inv_t, ts = a.stat[row * 4 + 3];
+    auto end = [&](const RowStat& st) {
+      if constexpr (FINISH) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what is replaced has been written
+        __syncthreads();
+        if (threadIdx.x < 64)
+          finish_row<T>(a, row, lds, st, JOIN && seg == 0,
+                        [&](int32_t col) { return wk.seg_of(z.vec_of(col), VPT) == seg; });
+        __syncthreads();
+      }
+    };
     if (wt == 0.f || ts == 0.f) {   // nothing flows into this row
       zero_segment<T, VPT>(z, out, wk, seg);
+      if (FINISH && JOIN && seg == 0) end(join_parts(a.part + row * a.S, a.S, a.c));
       continue;
     }
     const Segment<T, VPT> part(z, wk, seg);
@@ -718,140 +872,18 @@ __global__ __launch_bounds__(kThreads) void distill_grad(DistillArgs a) {
 #pragma unroll
       for (int k = 0; k < decltype(n)::value; ++k) x[k] = exp2_of(x[k], o, a.c) * scale;
     });
+    end(st);
   }
 }
 
-// A wave a row.  LOSS: the loss and the row's statistics.  With an output, what
-// distill_grad left at the teacher's entries is replaced by w (q - p) / T, the
-// p of equal columns summed in their order, rounded once.
-constexpr int kPlaceBits = 13, kRange = 32768;
-union FinishLds {   // of one wave
-  uint8_t place[1 << kPlaceBits];
-  struct {
-    uint32_t seen[kRange / 32], twice[kRange / 32];
-  } bits;
-};
-
+// A wave a row.  LOSS: from the rows' segments, else from their statistics.
 template <typename T, bool LOSS>
 __global__ __launch_bounds__(kThreads) void distill_finish(DistillArgs a) {
   __shared__ FinishLds lds[kThreads / 64];
-  FinishLds& s = lds[threadIdx.x >> 6];
-  const int lane = threadIdx.x & 63;
   for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.n; row += (int64_t)gridDim.x * 4) {
-    // what does not depend on the row pointer is on its way while that is read
-    const float tm = a.stat[row * 4 + 2], ts = a.stat[row * 4 + 3], wt = (a.weight ? a.weight[row] : 1.f) * a.inv_t;
-    int64_t b, e;
-    a.t.range(row, b, e);
-    // a lane's entry of the first 64 (most rows have no more) is read once
-    const bool has = b + lane < e;
-    const int32_t col0 = has ? a.t.col[b + lane] : -1;
-    const float val0 = has ? a.t.at(b + lane) : 0.f, x0 = has ? a.picked[b + lane] : 0.f;
-    auto entry = [&](int64_t i, int32_t& col, float& val) {
-      const bool first = i == b + lane;
-      col = first ? col0 : i < e ? a.t.col[i] : -1;
-      val = first ? val0 : i < e ? a.t.at(i) : 0.f;
-    };
-    const float l2t = log2_of(ts);
-    auto share_of = [&](int32_t col, float val) {
-      return col != -1 ? __builtin_amdgcn_exp2f((val - tm) * a.c - l2t) : 0.f;
-    };
-    RowStat st;
-    if (LOSS) {
-      st = join_parts(a.part + row * a.S, a.S, a.c);
-      const float o = origin(st.m), l2z = log2_of(st.z);
-      float loss = 0.f;
-      for (int64_t i = b + lane; i < e; i += 64) {
-        int32_t col;
-        float val;
-        entry(i, col, val);
-        if (col < 0 || col >= a.V) continue;
-        const float u = (val - tm) * a.c - l2t, p = __builtin_amdgcn_exp2f(u), x = i == b + lane ? x0 : a.picked[i];
-        if (!(p == 0.f)) loss += p * (kLn2 * u - ((x - o) * a.inv_t - kLn2 * l2z));
-      }
-      loss = wave_sum(loss);
-      if (ts != ts) loss = st.z = ts;   // a column outside the vocabulary, or a NaN
-      if (lane == 0) {
-        a.loss[row] = ts == 0.f ? 0.f : loss;   // (no mass: nothing to learn)
-        a.stat[row * 4] = st.m;
-        a.stat[row * 4 + 1] = st.z;
-      }
-    } else {
-      st = RowStat{a.stat[row * 4], a.stat[row * 4 + 1], 0.f};
-    }
-    if (!a.out || wt == 0.f || ts == 0.f) continue;
-    const float o = origin(st.m), scale = st.z == 0.f ? 0.f : wt / st.z;
-    T* out = static_cast<T*>(a.out) + row * a.ldo;
-    auto write = [&](int32_t col, float x, float p) {
-      out[col] = Elem<T>::cast(exp2_of(x, o, a.c) * scale - wt * p);
-    };
-    // the p of the row's entries whose column is a lane's, in order, and whether entry i, that lane's, is the first
-    auto search = [&](int64_t i, int32_t mine, float& p, bool& first) {
-      p = 0.f;
-      for (int64_t from = b; from < e; from += 64) {
-        int32_t col;
-        float val;
-        entry(from + lane, col, val);
-        const float share = share_of(col, val);
-        const int count = (int)(e - from < 64 ? e - from : 64), before = (int)(i - from < 64 ? i - from : 64);
-        for (int j = 0; j < count; ++j) {
-          const bool same = (int32_t)__builtin_amdgcn_readlane((uint32_t)col, j) == mine;
-          const float share_j = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(share), j));
-          p += same ? share_j : 0.f;
-          first = first && !(same && j < before);
-        }
-      }
-    };
-    if (e - b <= 64) {
-      // Equal columns meet in a table: the lane that is left in a place is done, one that finds its own column
-      // there has an equal, one that finds another's goes on (two rounds mostly; the search costs 5 us).
-      const bool mine = col0 >= 0 && col0 < a.V;
-      const uint32_t place = ((uint32_t)col0 * 0x9e3779b1u) >> (32 - kPlaceBits);
-      bool open = mine, equal = false;
-      while (__ballot(open) != 0 && __ballot(equal) == 0) {
-        if (open) s.place[place] = (uint8_t)lane;
-        wave_fence();
-        const int left = open ? (int)s.place[place] : lane;
-        wave_fence();
-        equal = __shfl(col0, left) == col0 && left != lane;
-        open = open && left != lane;
-      }
-      float p = share_of(col0, val0);
-      bool first = mine;
-      if (__ballot(equal) != 0) search(b + lane, col0, p, first);
-      if (first) write(col0, x0, p);
-      continue;
-    }
-    // More entries: a range of columns at a time, in one bit a column, or, where a few entries stand against many
-    // ranges, by searching for all of them.
-    const int64_t chunks = (e - b + 63) / 64, ranges = (a.V + kRange - 1) / kRange;
-    const bool by_range = ranges * (chunks + 3) <= 10 * chunks * chunks;
-    for (int64_t r = 0; r < (by_range ? ranges : 1); ++r) {
-      const int64_t lo = r * kRange, hi = by_range && lo + kRange < a.V ? lo + kRange : a.V;
-      if (by_range) {
-        for (int i = lane; i < kRange / 32; i += 64) s.bits.seen[i] = s.bits.twice[i] = 0u;
-        wave_fence();
-        for (int64_t i = b + lane; i < e; i += 64) {
-          const int32_t col = a.t.col[i];
-          if (col < lo || col >= hi) continue;
-          const int at = (int)(col - lo) >> 5;
-          const uint32_t bit = 1u << (col & 31);
-          if (atomicOr(&s.bits.seen[at], bit) & bit) atomicOr(&s.bits.twice[at], bit);
-        }
-        wave_fence();
-      }
-      for (int64_t base = b; base < e; base += 64) {
-        int32_t col;
-        float val;
-        entry(base + lane, col, val);
-        const bool mine = col >= lo && col < hi;
-        const bool equal = !by_range || (mine && ((s.bits.twice[(int)(col - lo) >> 5] >> (col & 31)) & 1));
-        float p = share_of(col, val);
-        bool first = mine;
-        if (__ballot(equal) != 0) search(base + lane, col, p, first);
-        if (first) write(col, a.picked[base + lane], p);
-      }
-      wave_fence();
-    }
+    const RowStat st = LOSS ? join_parts(a.part + row * a.S, a.S, a.c)
+                            : RowStat{a.stat[row * 4], a.stat[row * 4 + 1], 0.f};
+    finish_row<T>(a, row, lds[threadIdx.x >> 6], st, LOSS, [](int32_t) { return true; });
   }
 }
 
@@ -883,6 +915,21 @@ void with_vpt(int vpt, F&& f) {
   if constexpr (MOST > 1)
     if (vpt < MOST) return with_vpt<MOST / 2>(vpt, f);
   f(std::integral_constant<int, MOST>());
+}
+
+// The gradient's launches: one where its workgroups are on the chip all at once
+constexpr int64_t kFinishGroups = 2048;
+template <typename T, bool JOIN>
+void launch_grad(const DistillArgs& a, const Plan& q, hipStream_t s) {
+  const int64_t groups = a.n * q.wk.S;
+  const bool finish = groups <= kFinishGroups;
+  with_vpt<kGradPages>(q.vpt, [&](auto e) {
+    constexpr int E = decltype(e)::value;
+    auto kernel = finish ? distill_grad<T, E, JOIN, true> : distill_grad<T, E, JOIN, false>;
+    hipLaunchKernelGGL(kernel, dim3(groups_of(groups)), dim3(kThreads), 0, s, a);
+  });
+  if (!finish)
+    hipLaunchKernelGGL((distill_finish<T, JOIN>), dim3(groups_of((a.n + 3) / 4)), dim3(kThreads), 0, s, a);
 }
 
 // Threads a group whose maximum is kept for the alternatives: as many as leave
@@ -972,12 +1019,8 @@ SPMM_EXPORT int spmm_distill(const void* z, int64_t ld, int64_t n, int64_t V, in
       constexpr int E = decltype(e)::value;
       hipLaunchKernelGGL((distill_stats<T, E>), dim3(groups_of(n * p.wk.S + (n + 3) / 4)), dim3(kThreads), 0, s, sa, a);
     });
-    if (out)
-      with_vpt<kGradPages>(q.vpt, [&](auto e) {
-        constexpr int E = decltype(e)::value;
-        hipLaunchKernelGGL((distill_grad<T, E, true>), dim3(groups_of(n * q.wk.S)), dim3(kThreads), 0, s, a);
-      });
-    hipLaunchKernelGGL((distill_finish<T, true>), dim3(groups_of((n + 3) / 4)), dim3(kThreads), 0, s, a);
+    if (out) launch_grad<T, true>(a, q, s);
+    else hipLaunchKernelGGL((distill_finish<T, true>), dim3(groups_of((n + 3) / 4)), dim3(kThreads), 0, s, a);
     SPMM_LAUNCH_CHECK();
   });
   return 0;
@@ -994,11 +1037,7 @@ SPMM_EXPORT int spmm_distill_grad(const void* z, int64_t ld, int64_t n, int64_t 
   const DistillArgs a{z, ld, n, V, q.wk, c, inv_t, nullptr, 0, Teacher{rowptr, col, val, val_type, nnz}, nullptr,
                       const_cast<float*>(stat), const_cast<float*>(picked), weight, out, ldo};
   SPMM_VOCAB_TYPE(type, T, {
-    with_vpt<kGradPages>(q.vpt, [&](auto e) {
-      constexpr int E = decltype(e)::value;
-      hipLaunchKernelGGL((distill_grad<T, E, false>), dim3(groups_of(n * q.wk.S)), dim3(kThreads), 0, s, a);
-    });
-    hipLaunchKernelGGL((distill_finish<T, false>), dim3(groups_of((n + 3) / 4)), dim3(kThreads), 0, s, a);
+    launch_grad<T, false>(a, q, s);
     SPMM_LAUNCH_CHECK();
   });
   return 0;

@@ -44,7 +44,7 @@ _native.register_hip("spmm_distill_grad", c_vp, C.c_int64, C.c_int64, C.c_int64,
 
 @dataclass
 class DistillLoss:
-    loss: torch.Tensor       # fp32 [n]
+    loss: torch.Tensor       # fp32 [n], a part of `saved` (clone it to keep it alone)
     saved: torch.Tensor      # fp32: loss; per row the student's maximum and sum, the teacher's two; the student's
                              # logits at the teacher's entries; workspace
     rows: int

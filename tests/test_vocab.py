@@ -581,7 +581,7 @@ def test_distill(dev, dtype, n, V, most):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,V", [(300, 1000), (700, 2049), (530, 5001), (300, 20003)])
+@pytest.mark.parametrize("n,V", [(300, 1000), (700, 2049), (530, 5001), (300, 20003), (2500, 300)])
 def test_distill_many_rows(dtype, n, V):
     z, _ = logits(n, V, dtype, seed=14)
     w = torch.rand(n, generator=gen(15))
