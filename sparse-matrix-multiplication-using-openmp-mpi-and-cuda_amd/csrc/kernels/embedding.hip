@@ -766,6 +766,15 @@ bool grad_sizes(int64_t n, int64_t V, int64_t D, GradSizes& g) {
   return true;
 }
 
+// slices of a row of dY, 64 lanes' vectors each
+int64_t lane_slices(int64_t D, int in_type) {
+  const int64_t columns = 64 * (in_type == kF32 ? 4 : 8);
+  return (D + columns - 1) / columns;
+}
+bool is_brief(int64_t n, int64_t D, int in_type, int64_t ldw, int accumulate) {
+  return n <= kBriefTokens && n * lane_slices(D, in_type) <= kBriefGroups && D >= kNarrow && (accumulate || ldw == D);
+}
+
 template <typename TI, typename TO>
 int grad(GradArgs a, const void* tok, int wide, hipStream_t s) {
   if (a.brief) {
@@ -812,27 +821,27 @@ SPMM_EXPORT int spmm_embedding(const void* W, int64_t ldw, int64_t V, int64_t D,
   return 0;
 }
 
-// bytes of workspace, or -1 for sizes that the kernels do not take
-SPMM_EXPORT int64_t spmm_embedding_grad_ws(int64_t n, int64_t V, int64_t D) {
+// bytes of workspace, or -1 for sizes that the kernels do not take; ldw: row stride of the table
+SPMM_EXPORT int64_t spmm_embedding_grad_ws(int64_t n, int64_t V, int64_t D, int in_type, int64_t ldw, int accumulate) {
   GradSizes g;
-  return grad_sizes(n, V, D, g) ? g.total : -1;
+  if (!grad_sizes(n, V, D, g)) return -1;
+  return is_brief(n, D, in_type, ldw, accumulate) ? 0 : g.total;
 }
 
 SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, const void* tok, int wide, int64_t n,
                                     int64_t V, int64_t D, float scale, void* dw, int64_t ldw, int out_type,
                                     int accumulate, void* ws, int64_t ws_bytes, hipStream_t s) {
   GradSizes g;
-  if (!grad_sizes(n, V, D, g) || ws_bytes < g.total) return (int)hipErrorInvalidValue;
-  uint32_t* ka = static_cast<uint32_t*>(ws);
+  if (!grad_sizes(n, V, D, g)) return (int)hipErrorInvalidValue;
+  const bool brief = is_brief(n, D, in_type, ldw, accumulate);
+  if (!brief && ws_bytes < g.total) return (int)hipErrorInvalidValue;
+  uint32_t* ka = static_cast<uint32_t*>(ws);   // (all null in a brief call, which uses none of it)
   int32_t* pa = reinterpret_cast<int32_t*>(ka + g.keys);
   uint32_t* skey = ka;
   int32_t* spos = pa;
   int32_t* slot = accumulate ? nullptr : pa + g.keys;
   char* behind = reinterpret_cast<char*>(pa + g.keys + g.slots);
   int64_t zeroed = 0;   // bytes of the table that the sort's launch zeroes
-  const int lane_cols = in_type == kF32 ? 4 : 8;
-  const int64_t slices = (D + 64 * lane_cols - 1) / (64 * lane_cols);
-  const bool brief = n <= kBriefTokens && n * slices <= kBriefGroups && D >= kNarrow && (accumulate || ldw == D);
   if (brief) {
     // no sort
   } else if (n > kRankMax) {
@@ -886,7 +895,7 @@ SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, c
   a.part = reinterpret_cast<float*>(behind);
   a.accumulate = accumulate;
   a.zeroed = zeroed != 0;
-  a.slices = slices;
+  a.slices = lane_slices(D, in_type);
   a.brief = brief;
   SPMM_VOCAB_TYPE(in_type, TI, {
     if (out_type == kF32) return grad<TI, float>(a, tok, wide, s);

@@ -29,7 +29,8 @@ from . import rows as R
 
 _native.register_hip("spmm_embedding", c_vp, C.c_int64, C.c_int64, C.c_int64, C.c_int, c_vp, C.c_int, C.c_int64,
                      C.c_float, c_vp, C.c_int64, c_vp)
-_native.register_hip("spmm_embedding_grad_ws", C.c_int64, C.c_int64, C.c_int64, restype=C.c_int64)
+_native.register_hip("spmm_embedding_grad_ws", C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int64, C.c_int,
+                     restype=C.c_int64)
 _native.register_hip("spmm_embedding_grad", c_vp, C.c_int64, C.c_int, c_vp, C.c_int, C.c_int64, C.c_int64, C.c_int64,
                      C.c_float, c_vp, C.c_int64, C.c_int, C.c_int, c_vp, C.c_int64, c_vp)
 
@@ -122,13 +123,13 @@ def embedding_grad(dY: torch.Tensor, tokens: torch.Tensor, V: int, scale: float 
         out.copy_(acc)
         return out
     lib = _native.hip()
-    bytes_ = lib.spmm_embedding_grad_ws(n, V, D)
+    bytes_ = lib.spmm_embedding_grad_ws(n, V, D, R.TYPES[dy.dtype], out.stride(0), accumulate)
     if bytes_ < 0:
         raise ValueError(f"embedding_grad does not take {n} tokens over {V} rows")
     with R.on(dev):
-        ws = torch.empty(bytes_, dtype=torch.uint8, device=dev)
+        ws = torch.empty(bytes_, dtype=torch.uint8, device=dev) if bytes_ else None
         _native.check(lib.spmm_embedding_grad(dy.data_ptr(), dy.stride(0), R.TYPES[dy.dtype], tok.data_ptr(),
                                               tok.dtype == torch.int64, n, V, D, scale, out.data_ptr(), out.stride(0),
-                                              R.TYPES[dtype], accumulate, ws.data_ptr(), bytes_,
+                                              R.TYPES[dtype], accumulate, ws.data_ptr() if bytes_ else None, bytes_,
                                               _native.stream_ptr(dev)), "embedding_grad")
     return out

@@ -39,6 +39,7 @@ _native.register_hip("spmm_token_logprobs_grad", c_vp, C.c_int64, C.c_int64, C.c
                      C.c_float, C.c_float, c_vp, c_vp, c_vp, c_vp, C.c_int64, c_vp)
 
 MAX_TOP = 128   # vocab_logits.hip kMaxTop
+KEPT = 1 << 16  # bytes of workspace that live on with the result, which saves an allocation of 1.8 us
 LOG2E = 1.0 / math.log(2.0)
 
 
@@ -46,7 +47,7 @@ LOG2E = 1.0 / math.log(2.0)
 class TokenLogprobs:
     logprob: torch.Tensor    # fp32 [n]
     entropy: torch.Tensor    # fp32 [n]
-    stat: torch.Tensor       # fp32 [4, n]: both, the row's maximum m and its sum of exp((z - m) / T)
+    stat: torch.Tensor       # fp32 [>= 4, n]: both, the row's maximum m and its sum of exp((z - m) / T); workspace
     temperature: float
     top: Optional[CSR]       # n x V, k entries a row, largest first (fp32 log-probabilities)
 
@@ -84,8 +85,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     k = int(k)
     if not 0 <= k <= min(MAX_TOP, V):
         raise ValueError(f"k must be between 0 and {min(MAX_TOP, V)}, got {k}")
-    stat = torch.empty((4, n), dtype=torch.float32, device=dev)
-    logprob, entropy, _, _ = stat.unbind(0)
+    gpu = dev.type == "cuda" and n > 0
+    bytes_ = _native.hip().spmm_vocab_ws(n, V, R.TYPES[z.dtype], k) if gpu else 0
+    kept = bytes_ <= KEPT   # (a row's workspace is whole floats, and starts at 16 bytes)
+    stat = torch.empty((4 + (bytes_ // (4 * n) if gpu and kept else 0), n), dtype=torch.float32, device=dev)
+    logprob, entropy = stat[0], stat[1]
     top = None
     if k:
         top = CSR(n, V, torch.empty(n + 1, dtype=torch.int64, device=dev),
@@ -104,14 +108,13 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
         _native.check(_native.host().spmm_cpu_token_logprobs(n, V, zf.data_ptr(), t.data_ptr(), inv_t, k,
                                                              stat.data_ptr(), at[1], at[2], 0), "cpu_token_logprobs")
         return res
-    lib = _native.hip()
-    code = R.TYPES[z.dtype]
-    bytes_ = lib.spmm_vocab_ws(n, V, code, k)
     with R.on(dev):
-        ws = torch.empty(bytes_, dtype=torch.uint8, device=dev)
-        _native.check(lib.spmm_token_logprobs(
-            z.data_ptr(), z.stride(0), n, V, code, tok.data_ptr(), tok.dtype == torch.int64, k, LOG2E * inv_t, inv_t,
-            stat.data_ptr(), *at, ws.data_ptr(), bytes_, _native.stream_ptr(dev)), "token_logprobs")
+        at_stat = stat.data_ptr()
+        ws = None if kept else torch.empty(bytes_, dtype=torch.uint8, device=dev)
+        _native.check(_native.hip().spmm_token_logprobs(
+            z.data_ptr(), z.stride(0), n, V, R.TYPES[z.dtype], tok.data_ptr(), tok.dtype == torch.int64, k,
+            LOG2E * inv_t, inv_t, at_stat, *at, at_stat + 16 * n if kept else ws.data_ptr(), bytes_,
+            _native.stream_ptr(dev)), "token_logprobs")
     return res
 
 
@@ -131,8 +134,13 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: Token
     R.same_device(dev, tokens=tokens, g_logprob=g_logprob, g_entropy=g_entropy, stats=stats.stat)
     if tokens.dim() != 1 or tokens.shape[0] != n:
         raise ValueError(f"tokens must be [{n}], got {tuple(tokens.shape)}")
-    if stats.stat.shape[1] != n:
-        raise ValueError(f"stats are of {stats.stat.shape[1]} rows, the logits have {n}")
+    stat = stats.stat
+    if stat.dtype != torch.float32 or stat.dim() != 2 or stat.shape[0] < 4:
+        raise ValueError(f"stats must be fp32 [4, {n}], got {stat.dtype} {tuple(stat.shape)}")
+    if stat.shape[1] != n:
+        raise ValueError(f"stats are of {stat.shape[1]} rows, the logits have {n}")
+    if not stat.is_contiguous():   # (some of a larger batch's rows)
+        stat = stat.contiguous()
     tok = R.token_ids(tokens)
     g, h = R.per_row(g_logprob, n, "g_logprob"), R.per_row(g_entropy, n, "g_entropy")
     inv_t = R.inverse_temperature(stats.temperature)
@@ -145,13 +153,13 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: Token
         zf, t = z.float().contiguous(), tok.to(torch.int64)
         acc = torch.empty((n, V), dtype=torch.float32)
         _native.check(_native.host().spmm_cpu_token_logprobs_grad(n, V, zf.data_ptr(), t.data_ptr(), inv_t,
-                                                                  stats.stat.data_ptr(), at_g, at_h, acc.data_ptr(), 0),
+                                                                  stat.data_ptr(), at_g, at_h, acc.data_ptr(), 0),
                       "cpu_token_logprobs_grad")
         out.copy_(acc)
         return out
     with R.on(dev):
         _native.check(_native.hip().spmm_token_logprobs_grad(
             z.data_ptr(), z.stride(0), n, V, R.TYPES[z.dtype], tok.data_ptr(), tok.dtype == torch.int64, LOG2E * inv_t,
-            inv_t, stats.stat.data_ptr(), at_g, at_h, out.data_ptr(), out.stride(0), _native.stream_ptr(dev)),
+            inv_t, stat.data_ptr(), at_g, at_h, out.data_ptr(), out.stride(0), _native.stream_ptr(dev)),
             "token_logprobs_grad")
     return out

@@ -9,6 +9,7 @@ sum of magnitudes.  Each term exp2(u) is off by 2^-23 (the instruction) plus
 |u| 2^-23 (u is rounded once, its factor log2(e) / T once): below 60 2^-24
 weighted by the term, whose u above -30 alone counts.  SUM covers them.
 """
+import dataclasses
 import math
 
 import pytest
@@ -371,7 +372,7 @@ def test_more_rows_than_workgroups():
     tok = torch.randint(0, V, (n,), generator=gen(35)).cuda()
     g = torch.rand(n, generator=gen(36)).cuda()
     a, b = token_logprobs(z, tok, k=3), token_logprobs(z[-last:], tok[-last:], k=3)
-    assert torch.equal(a.stat[:, -last:], b.stat)
+    assert torch.equal(a.stat[:4, -last:], b.stat[:4])
     assert torch.equal(a.top.col[-3 * last:], b.top.col) and torch.equal(a.top.val[-3 * last:], b.top.val)
     dz = token_logprobs_grad(z, tok, a, g, g)
     assert torch.equal(dz[-last:], token_logprobs_grad(z[-last:], tok[-last:], b, g[-last:], g[-last:]))
@@ -470,6 +471,18 @@ def test_logprobs_grad_masks(dev):
     h[4] = 0.0                       # a padded row of garbage: nothing flows, nothing is read
     got = check_token_grad(z, tok, g, h, 1.5, dev)
     assert (got[4] == 0).all() and got[6].isnan().all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_logprobs_grad_of_some_rows(dev):
+    """The statistics of a batch, cut like its logits: a gradient by parts."""
+    z, tok = logits(9, 700, torch.bfloat16, seed=39)
+    z, tok, g = z.to(dev), tok.to(dev), torch.randn(9, generator=gen(40)).to(dev)
+    r = token_logprobs(z, tok, temperature=1.5)
+    whole = token_logprobs_grad(z, tok, r, g, g)
+    for lo, hi in ((0, 4), (4, 9), (3, 4)):
+        part = dataclasses.replace(r, stat=r.stat[:, lo:hi])
+        assert torch.equal(token_logprobs_grad(z[lo:hi], tok[lo:hi], part, g[lo:hi], g[lo:hi]), whole[lo:hi])
 
 
 @pytest.mark.parametrize("dev", DEVICES)
