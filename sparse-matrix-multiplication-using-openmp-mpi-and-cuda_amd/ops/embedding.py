@@ -8,8 +8,8 @@ arrays, takes fp32, bf16 and fp16 and any width, and reads every row once.
 * Token -1 is padding: its row of Y is zero and it adds nothing to dW.
 * A token that the table does not have (below -1, or V and above) gives a row
   of NaN and adds nothing to dW: checking it on the host would wait for the GPU.
-* Sums are held in fp32 over ascending positions whatever the launch, and
-  rounded once: results are the same in every run.
+* Sums are held in fp32, over ascending positions in parts that the sizes
+  determine, and rounded once: results are the same in every run.
 
 gfx950 kernels: ``csrc/kernels/embedding.hip``; CPU tensors use the OpenMP
 kernels of ``csrc/host/vocab_cpu.cpp``.  Nothing here waits for the GPU, so
