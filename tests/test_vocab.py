@@ -800,6 +800,30 @@ def test_captured_and_replayed():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 1500, 13000])
+def test_captured_gradients(n):
+    """Every way of the table's gradient in a graph: unsorted, sorted in one launch, in several."""
+    dev, V, D = torch.device("cuda"), 4001, 72
+    dY, tok = torch.randn(n, D, device=dev).bfloat16(), torch.randint(0, V, (n,), device=dev)
+    main = torch.zeros(V, D, device=dev)
+    embedding_grad(dY, tok, V)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        dW = embedding_grad(dY, tok, V)
+        embedding_grad(dY, tok, V, out=main, accumulate=True)
+    total = torch.zeros(V, D, device=dev)
+    for i in range(4):
+        dY.copy_(torch.randn(n, D, device=dev).bfloat16())
+        tok.copy_(torch.randint(-1, V, (n,), device=dev))
+        gr.replay()
+        assert torch.equal(dW, embedding_grad(dY, tok, V))
+        embedding_grad(dY, tok, V, out=total, accumulate=True)
+        assert torch.equal(main, total)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
 def test_on_another_stream():
     dev = torch.device("cuda")
     W, tok = torch.randn(3000, 200, device=dev), torch.randint(0, 3000, (9000,), device=dev)
