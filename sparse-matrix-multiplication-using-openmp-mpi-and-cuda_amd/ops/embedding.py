@@ -58,7 +58,7 @@ def embedding(W: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
     V, D = W.shape
     n = tok.numel()
     if out is None:
-        out = torch.empty((*tokens.shape, D), dtype=W.dtype, device=dev)
+        out = torch.empty(*tokens.shape, D, dtype=W.dtype, device=dev)   # (a tuple costs 0.4 us more)
     else:
         R.no_grad_of("embedding_grad", out)
         R.output(out, (*tokens.shape, D), W.dtype, dev)
@@ -109,7 +109,7 @@ def embedding_grad(dY: torch.Tensor, tokens: torch.Tensor, V: int, scale: float 
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs the out that it adds to")
-        out = torch.empty((V, D), dtype=dtype, device=dev)
+        out = torch.empty(V, D, dtype=dtype, device=dev)
     else:
         R.output(out, (V, D), dtype, dev)
         R.apart(out, dy, "dY", in_place=False)

@@ -62,7 +62,7 @@ def logits_rows(logits: torch.Tensor) -> torch.Tensor:
 def gradient_out(out: Optional[torch.Tensor], z: torch.Tensor) -> torch.Tensor:
     """A new gradient of z's shape and type, or the caller's (z itself allowed)."""
     if out is None:
-        return torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        return torch.empty(*z.shape, dtype=z.dtype, device=z.device)
     R.output(out, z.shape, z.dtype, z.device)
     R.apart(out, z, "logits", in_place=True)
     return out
@@ -88,7 +88,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     gpu = dev.type == "cuda" and n > 0
     bytes_ = _native.hip().spmm_vocab_ws(n, V, R.TYPES[z.dtype], k) if gpu else 0
     kept = bytes_ <= KEPT   # (a row's workspace is whole floats, and starts at 16 bytes)
-    stat = torch.empty((4 + (bytes_ // (4 * n) if gpu and kept else 0), n), dtype=torch.float32, device=dev)
+    stat = torch.empty(4 + (bytes_ // (4 * n) if gpu and kept else 0), n, dtype=torch.float32, device=dev)
     logprob, entropy = stat[0], stat[1]
     top = None
     if k:

@@ -110,6 +110,6 @@ def inverse_temperature(temperature: float) -> float:
 
 def on(device: torch.device):
     """Launches go to the current device: make it the operands'."""
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         return _NOTHING
     return torch.cuda.device(device)
