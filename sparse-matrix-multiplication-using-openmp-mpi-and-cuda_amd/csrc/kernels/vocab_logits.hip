@@ -122,9 +122,9 @@ struct StatsArgs {
   int lanes;        // a group: 1, 2, 4, 8, 16 or 64 neighbouring threads of a workgroup
 };
 
-// The statistics of segment t % S of row t / S, by one workgroup.
+// The statistics of segment t % S of row t / S, by one workgroup (thread 0 has them).
 template <typename T, int VPT, bool ENT, bool TOP>
-__device__ __forceinline__ void segment_stats(const StatsArgs& a, int64_t t, float* red) {
+__device__ __forceinline__ Part segment_stats(const StatsArgs& a, int64_t t, float* red) {
   constexpr int N = Elem<T>::kN;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const Walk wk = a.wk;
@@ -181,8 +181,7 @@ __device__ __forceinline__ void segment_stats(const StatsArgs& a, int64_t t, flo
       red[8 + w] = uw;
     }
     __syncthreads();
-    if (tid == 0)
-      a.part[t] = Part{m, (red[4] + red[5]) + (red[6] + red[7]), (red[8] + red[9]) + (red[10] + red[11]), 0.f};
+    const Part part{m, (red[4] + red[5]) + (red[6] + red[7]), (red[8] + red[9]) + (red[10] + red[11]), 0.f};
     if constexpr (TOP) {
       uint32_t key = key_of(mx);
       if (!(zs < kInf)) {   // a NaN among this thread's elements, or +inf
@@ -198,13 +197,17 @@ __device__ __forceinline__ void segment_stats(const StatsArgs& a, int64_t t, flo
       if ((tid & (a.lanes - 1)) == 0) a.keys[t * (kThreads / a.lanes) + tid / a.lanes] = key;
     }
     __syncthreads();   // red is written again
+    return part;
   }
 }
 
 template <typename T, int VPT, bool TOP>
 __global__ __launch_bounds__(kThreads) void vocab_stats(StatsArgs a) {
   __shared__ float red[12];
-  for (int64_t t = blockIdx.x; t < a.n * a.wk.S; t += gridDim.x) segment_stats<T, VPT, true, TOP>(a, t, red);
+  for (int64_t t = blockIdx.x; t < a.n * a.wk.S; t += gridDim.x) {
+    const Part part = segment_stats<T, VPT, true, TOP>(a, t, red);
+    if (threadIdx.x == 0) a.part[t] = part;
+  }
 }
 
 // A row's segments put together by one wave (all lanes get the result).
@@ -480,25 +483,54 @@ __device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& 
   wave_fence();
 }
 
+// A row's token: its number and its logit.
+struct Token {
+  int64_t id;
+  float x;
+  bool inside;
+};
+template <typename T>
+__device__ __forceinline__ Token token_of(const JoinArgs& a, int64_t row) {
+  Token t;
+  t.id = token_at(a.tok, a.wide, row);
+  t.inside = t.id >= 0 && t.id < a.wk.V;
+  t.x = Elem<T>::load(static_cast<const T*>(a.z) + row * a.ld + (t.inside ? t.id : 0));
+  return t;
+}
+
+// ln q of a row's logit y
+__device__ __forceinline__ float ln_q_of(const JoinArgs& a, const RowStat& st, float y) {
+  return (y - origin(st.m)) * a.inv_t - kLn2 * log2_of(st.z);
+}
+
+// a row's four results, by one thread
+__device__ __forceinline__ void write_stat(const JoinArgs& a, int64_t row, const RowStat& st, const Token& t) {
+  a.stat[row] = t.inside ? ln_q_of(a, st, t.x) : t.id == -1 ? 0.f : __builtin_nanf("");   // (-1: padding)
+  a.stat[a.n + row] = st.z == 0.f ? 0.f : kLn2 * (log2_of(st.z) - st.u / st.z);
+  a.stat[2 * a.n + row] = st.m;
+  a.stat[3 * a.n + row] = st.z;
+}
+
+// Rows that one workgroup holds, without alternatives: all in one launch.
+template <typename T, int VPT>
+__global__ __launch_bounds__(kThreads) void vocab_rows(StatsArgs s, JoinArgs a) {
+  __shared__ float red[12];
+  for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+    const Token token = token_of<T>(a, row);
+    const Part p = segment_stats<T, VPT, true, false>(s, row, red);
+    if (threadIdx.x == 0) write_stat(a, row, RowStat{p.m, p.z < kInf ? p.z : __builtin_nanf(""), p.u}, token);
+  }
+}
+
 // A wave a row.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void vocab_join(JoinArgs a) {
   __shared__ std::conditional_t<TOP, TopLds, int> top[4];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   for (int64_t row = (int64_t)blockIdx.x * 4 + w; row < a.n; row += (int64_t)gridDim.x * 4) {
-    const T* z = static_cast<const T*>(a.z) + row * a.ld;
-    const int64_t id = token_at(a.tok, a.wide, row);
-    const bool inside = id >= 0 && id < a.wk.V;
-    const float x = Elem<T>::load(z + (inside ? id : 0));
+    const Token token = token_of<T>(a, row);
     const RowStat st = join_parts(a.part + row * a.wk.S, a.wk.S, a.c);
-    const float o = origin(st.m), l2z = log2_of(st.z);
-    auto ln_q = [&](float y) { return (y - o) * a.inv_t - kLn2 * l2z; };
-    if (lane == 0) {
-      a.stat[row] = inside ? ln_q(x) : id == -1 ? 0.f : __builtin_nanf("");   // (-1: padding)
-      a.stat[a.n + row] = st.z == 0.f ? 0.f : kLn2 * (l2z - st.u / st.z);
-      a.stat[2 * a.n + row] = st.m;
-      a.stat[3 * a.n + row] = st.z;
-    }
+    if (lane == 0) write_stat(a, row, st, token);
     if constexpr (TOP) {
       if (lane == 0) {
         a.rowptr[row] = row * a.k;
@@ -506,7 +538,7 @@ __global__ __launch_bounds__(kThreads) void vocab_join(JoinArgs a) {
       }
       row_top<T>(a, row, top[w], [&](int place, uint64_t e) {
         a.top_col[row * a.k + place] = col_of(e);
-        a.top_val[row * a.k + place] = ln_q(value_of((uint32_t)(e >> 32)));
+        a.top_val[row * a.k + place] = ln_q_of(a, st, value_of((uint32_t)(e >> 32)));
       });
     }
   }
@@ -686,7 +718,8 @@ __global__ __launch_bounds__(kThreads) void distill_stats(StatsArgs s, DistillAr
   const int64_t segments = a.n * s.wk.S, groups = segments + (a.n + 3) / 4;
   for (int64_t t = blockIdx.x; t < groups; t += gridDim.x) {
     if (t < segments) {
-      segment_stats<T, VPT, false, false>(s, t, red);
+      const Part part = segment_stats<T, VPT, false, false>(s, t, red);
+      if (threadIdx.x == 0) s.part[t] = part;
     } else {
       const int64_t row = (t - segments) * 4 + (threadIdx.x >> 6);
       if (row < a.n) pick_row<T>(a, row);
@@ -948,7 +981,7 @@ int group_lanes(int64_t S, int k) {
 
 }  // namespace
 
-// bytes of workspace of spmm_token_logprobs (k >= 0) and of the distillation (k = 0)
+// bytes of workspace of spmm_token_logprobs and (k = 0) of the distillation
 SPMM_EXPORT int64_t spmm_vocab_ws(int64_t n, int64_t V, int type, int k) {
   if (!sizes_ok(n, V, type) || k < 0 || k > kMaxTop || k > V) return -1;
   const int64_t S = plan(n, V, type, kStatsPages).wk.S;
@@ -961,7 +994,7 @@ SPMM_EXPORT int spmm_token_logprobs(const void* z, int64_t ld, int64_t n, int64_
   const int64_t need = spmm_vocab_ws(n, V, type, k);
   if (need < 0 || ws_bytes < need) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
-  const Plan p = plan(n, V, type, kStatsPages);
+  const Plan p = plan(n, V, type, kStatsPages), whole = plan(kFill, V, type, kStatsPages);
   const int64_t S = p.wk.S;
   Part* part = static_cast<Part*>(ws);
   uint32_t* keys = reinterpret_cast<uint32_t*>(part + n * S);
@@ -969,6 +1002,14 @@ SPMM_EXPORT int spmm_token_logprobs(const void* z, int64_t ld, int64_t n, int64_
   const StatsArgs sa{z, ld, n, p.wk, c, part, keys, lanes};
   const JoinArgs ja{z, ld, n, p.wk, p.vpt, c, inv_t, part, tok, wide, k, lanes, keys, stat, rowptr, top_col, top_val};
   SPMM_VOCAB_TYPE(type, T, {
+    if (k == 0 && whole.wk.S == 1) {
+      const StatsArgs ra{z, ld, n, whole.wk, c, nullptr, nullptr, 1};
+      with_vpt<kStatsPages>(whole.vpt, [&](auto e) {
+        hipLaunchKernelGGL((vocab_rows<T, decltype(e)::value>), dim3(groups_of(n)), dim3(kThreads), 0, s, ra, ja);
+      });
+      SPMM_LAUNCH_CHECK();
+      return 0;
+    }
     with_vpt<kStatsPages>(p.vpt, [&](auto e) {
       constexpr int E = decltype(e)::value;
       if (k) hipLaunchKernelGGL((vocab_stats<T, E, true>), dim3(groups_of(n * S)), dim3(kThreads), 0, s, sa);
