@@ -122,7 +122,7 @@ struct StatsArgs {
   int lanes;        // a group: 1, 2, 4, 8, 16 or 64 neighbouring threads of a workgroup
 };
 
-// The statistics of segment t % S of row t / S, by one workgroup (thread 0 has them).
+// The statistics of segment t % S of row t / S, by one workgroup (all threads get them).
 template <typename T, int VPT, bool ENT, bool TOP>
 __device__ __forceinline__ Part segment_stats(const StatsArgs& a, int64_t t, float* red) {
   constexpr int N = Elem<T>::kN;
@@ -855,7 +855,28 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, Fi
   }
 }
 
-// w q / T everywhere.  JOIN: the rows' statistics are put together here, from
+// w q / T in a segment of a row; stat(): the row's statistics, asked for behind
+// the loads.  False: nothing flows into the row, which is zero.
+template <typename T, int VPT, typename F>
+__device__ __forceinline__ bool write_grad(const DistillArgs& a, const Walk& wk, int64_t row, int seg, F&& stat) {
+  const Row<T> z(a.z, a.ld, row, wk.V);
+  T* out = static_cast<T*>(a.out) + row * a.ldo;
+  const float wt = (a.weight ? a.weight[row] : 1.f) * a.inv_t, ts = a.stat[row * 4 + 3];
+  if (wt == 0.f || ts == 0.f) {
+    zero_segment<T, VPT>(z, out, wk, seg);
+    return false;
+  }
+  const Segment<T, VPT> part(z, wk, seg);
+  const RowStat st = stat();
+  const float o = origin(st.m), scale = ts != ts ? ts : st.z == 0.f ? 0.f : wt / st.z;
+  part.write(z, out, wk, seg, [&](float* x, int, auto n) {
+#pragma unroll
+    for (int k = 0; k < decltype(n)::value; ++k) x[k] = exp2_of(x[k], o, a.c) * scale;
+  });
+  return true;
+}
+
+// The same everywhere.  JOIN: the rows' statistics are put together here, from
 // their segments'.
 //
 // Bytes bound a step of loss and gradient: the logits are read twice and the
@@ -878,34 +899,27 @@ __global__ __launch_bounds__(kThreads) void distill_grad(DistillArgs a) {
   for (int64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
     const int64_t row = t / wk.S;
     const int seg = (int)(t - row * wk.S);
-    const Row<T> z(a.z, a.ld, row, wk.V);
-    T* out = static_cast<T*>(a.out) + row * a.ldo;
-    const float wt = (a.weight ? a.weight[row] : 1.f) * a.inv_t, ts = a.stat[row * 4 + 3];
-    auto end = [&](const RowStat& st) {
-      if constexpr (FINISH) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what is replaced has been written
-        __syncthreads();
-        if (threadIdx.x < 64)
-          finish_row<T>(a, row, lds, st, JOIN && seg == 0,
-                        [&](int32_t col) { return wk.seg_of(z.vec_of(col), VPT) == seg; });
-        __syncthreads();
-      }
-    };
-    if (wt == 0.f || ts == 0.f) {   // nothing flows into this row
-      zero_segment<T, VPT>(z, out, wk, seg);
-      if (FINISH && JOIN && seg == 0) end(join_parts(a.part + row * a.S, a.S, a.c));
-      continue;
-    }
-    const Segment<T, VPT> part(z, wk, seg);
     RowStat st;
-    if (JOIN) st = join_parts(a.part + row * a.S, a.S, a.c);
-    else st = RowStat{a.stat[row * 4], a.stat[row * 4 + 1], 0.f};
-    const float o = origin(st.m), scale = ts != ts ? ts : st.z == 0.f ? 0.f : wt / st.z;
-    part.write(z, out, wk, seg, [&](float* x, int, auto n) {
-#pragma unroll
-      for (int k = 0; k < decltype(n)::value; ++k) x[k] = exp2_of(x[k], o, a.c) * scale;
-    });
-    end(st);
+    auto stat = [&] {
+      if (JOIN) st = join_parts(a.part + row * a.S, a.S, a.c);
+      else st = RowStat{a.stat[row * 4], a.stat[row * 4 + 1], 0.f};
+      return st;
+    };
+    const bool flows = write_grad<T, VPT>(a, wk, row, seg, stat);
+    if constexpr (FINISH) {
+      if (!flows) {
+        if (!JOIN || seg != 0) continue;   // (the loss is still to be written)
+        stat();
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what is replaced has been written
+      __syncthreads();
+      if (threadIdx.x < 64) {
+        const Row<T> z(a.z, a.ld, row, wk.V);
+        finish_row<T>(a, row, lds, st, JOIN && seg == 0,
+                      [&](int32_t col) { return wk.seg_of(z.vec_of(col), VPT) == seg; });
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -917,6 +931,29 @@ __global__ __launch_bounds__(kThreads) void distill_finish(DistillArgs a) {
     const RowStat st = LOSS ? join_parts(a.part + row * a.S, a.S, a.c)
                             : RowStat{a.stat[row * 4], a.stat[row * 4 + 1], 0.f};
     finish_row<T>(a, row, lds[threadIdx.x >> 6], st, LOSS, [](int32_t) { return true; });
+  }
+}
+
+// Rows that one workgroup holds: loss, statistics and, with an output, the
+// gradient in one launch, which reads its logits again out of the caches.  Its
+// steps wait for each other: where the rows fill the chip it pays if they are
+// long and the second read counts (loss and gradient of 256 x 16000 bf16 9.6 us
+// instead of 14.4, 1000 x 5000 fp32 14.0 instead of 25.9, 8000 x 16000 139
+// instead of 192, but 8000 x 1300 51 instead of 46; loss alone of 48 x 8000 fp16
+// 5.5 instead of 6.2, of 2000 x 8000 14.4 instead of 12.3).
+template <typename T, int VPT>
+__global__ __launch_bounds__(kThreads) void distill_rows(StatsArgs s, DistillArgs a) {
+  __shared__ float red[12];
+  __shared__ FinishLds lds;
+  for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+    if (threadIdx.x < 64) pick_row<T>(a, row);
+    const Part p = segment_stats<T, VPT, false, false>(s, row, red);   // (ends with a barrier)
+    const RowStat st{p.m, p.z < kInf ? p.z : __builtin_nanf(""), 0.f};
+    if (a.out) write_grad<T, VPT>(a, s.wk, row, 0, [&] { return st; });
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what is replaced has been written
+    __syncthreads();
+    if (threadIdx.x < 64) finish_row<T>(a, row, lds, st, true, [](int32_t) { return true; });
+    __syncthreads();
   }
 }
 
@@ -949,6 +986,8 @@ void with_vpt(int vpt, F&& f) {
     if (vpt < MOST) return with_vpt<MOST / 2>(vpt, f);
   f(std::integral_constant<int, MOST>());
 }
+
+constexpr int64_t kFewRows = 1024;   // of distill_rows whatever their length
 
 // The gradient's launches: one where its workgroups are on the chip all at once
 constexpr int64_t kFinishGroups = 2048;
@@ -1053,9 +1092,18 @@ SPMM_EXPORT int spmm_distill(const void* z, int64_t ld, int64_t n, int64_t V, in
   const Plan p = plan(n, V, type, kStatsPages), q = plan(n, V, type, kGradPages);
   Part* part = static_cast<Part*>(ws);
   const StatsArgs sa{z, ld, n, p.wk, c, part, nullptr, 1};
+  const Plan whole = plan(kFill, V, type, kStatsPages);
   const DistillArgs a{z, ld, n, V, q.wk, c, inv_t, part, p.wk.S, Teacher{rowptr, col, val, val_type, nnz}, loss, stat,
                       picked, weight, out, ldo};
   SPMM_VOCAB_TYPE(type, T, {
+    if (whole.wk.S == 1 && (n <= kFewRows || (out && whole.vpt == kStatsPages))) {
+      const StatsArgs ra{z, ld, n, whole.wk, c, nullptr, nullptr, 1};
+      with_vpt<kStatsPages>(whole.vpt, [&](auto e) {
+        hipLaunchKernelGGL((distill_rows<T, decltype(e)::value>), dim3(groups_of(n)), dim3(kThreads), 0, s, ra, a);
+      });
+      SPMM_LAUNCH_CHECK();
+      return 0;
+    }
     with_vpt<kStatsPages>(p.vpt, [&](auto e) {
       constexpr int E = decltype(e)::value;
       hipLaunchKernelGGL((distill_stats<T, E>), dim3(groups_of(n * p.wk.S + (n + 3) / 4)), dim3(kThreads), 0, s, sa, a);
