@@ -18,7 +18,8 @@
 //          largest logit: only the k groups or so that reach it are read again.
 // grad     reads a segment again and writes its gradient.
 // Long rows of few tokens are split over many workgroups like this, many rows
-// fill the chip the same way; the logits' bytes bound all three.
+// fill the chip the same way; the logits' bytes bound all three.  Rows that fit
+// the registers of a workgroup take one launch: vocab_rows, distill_rows.
 #include "vocab_common.hpp"
 
 using namespace spmm;
@@ -231,6 +232,87 @@ __device__ __forceinline__ RowStat join_parts(const Part* p, int64_t S, float c)
   z = wave_sum(z);
   return RowStat{m, z < kInf ? z : __builtin_nanf(""), wave_sum(u)};   // (+inf among the logits)
 }
+
+// A row in the registers of a workgroup, and its statistics.
+template <typename T, int VPT, int THREADS>
+struct HeldRow {
+  static constexpr int N = Elem<T>::kN, kWaves = THREADS / 64;
+  u32x4 r[VPT];
+  float tail;
+  int extra;
+  __device__ __forceinline__ explicit HeldRow(const Row<T>& z) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      r[j] = u32x4{Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf};
+      if (j * THREADS + tid < z.nv) r[j] = z.vec(j * THREADS + tid);
+    }
+    extra = z.extra(tid);
+    tail = extra >= 0 ? Elem<T>::load(z.z + extra) : -kInf;
+  }
+  // red: 3 kWaves floats in LDS, which a barrier behind this call separates from their next use.  ENT: U too
+  template <bool ENT>
+  __device__ __forceinline__ RowStat stats(const Row<T>& z, float c, float* red) const {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    typename Elem<T>::Max most;
+    most.one(tail);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) most.vec(r[j]);
+    const float wm = wave_max(most.get());
+    if (lane == 0) red[w] = wm;
+    __syncthreads();
+    RowStat st{red[0], 0.f, 0.f};
+#pragma unroll
+    for (int q = 1; q < kWaves; ++q) st.m = fmaxf(st.m, red[q]);
+    const float o = origin(st.m);
+    float zs = 0.f, us = 0.f;
+    auto sum = [&](auto masked) {
+      zs = us = 0.f;
+      auto add = [&](float x) {
+        const float u = (x - o) * c, e = __builtin_amdgcn_exp2f(u);
+        zs += e;
+        if (ENT) us = __builtin_fmaf(e, decltype(masked)::value ? fmaxf(u, -1e30f) : u, us);
+      };
+      if (extra >= 0) add(tail);
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        if (j * THREADS >= z.nv) break;
+        if (j * THREADS + (int)threadIdx.x < z.nv) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) add(Elem<T>::get(r[j], i));
+        }
+      }
+    };
+    sum(std::false_type());
+    if (ENT && __ballot(us != us)) sum(std::true_type());   // (0 times -inf, as in segment_stats)
+    zs = wave_sum(zs);
+    us = ENT ? wave_sum(us) : 0.f;
+    if (lane == 0) {
+      red[kWaves + w] = zs;
+      red[2 * kWaves + w] = us;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kWaves; ++q) {
+      st.z += red[kWaves + q];
+      st.u += red[2 * kWaves + q];
+    }
+    st.z = st.z < kInf ? st.z : __builtin_nanf("");
+    return st;
+  }
+};
+
+// f(vectors a thread, threads) for rows of up to 32 pages
+template <typename F>
+void with_rows(int64_t pages, F&& f) {
+  if (pages > 16) f(std::integral_constant<int, 8>(), std::integral_constant<int, 1024>());
+  else if (pages > 8) f(std::integral_constant<int, 8>(), std::integral_constant<int, 512>());
+  else if (pages > 4) f(std::integral_constant<int, 8>(), std::integral_constant<int, 256>());
+  else if (pages > 2) f(std::integral_constant<int, 4>(), std::integral_constant<int, 256>());
+  else if (pages > 1) f(std::integral_constant<int, 2>(), std::integral_constant<int, 256>());
+  else f(std::integral_constant<int, 1>(), std::integral_constant<int, 256>());
+}
+int64_t pages_of(int64_t V, int type) { return (V / (type == kF32 ? 4 : 8) + kThreads - 1) / kThreads; }
 
 // ---- log-probabilities ------------------------------------------------------------
 
@@ -512,13 +594,15 @@ __device__ __forceinline__ void write_stat(const JoinArgs& a, int64_t row, const
 }
 
 // Rows that one workgroup holds, without alternatives: all in one launch.
-template <typename T, int VPT>
-__global__ __launch_bounds__(kThreads) void vocab_rows(StatsArgs s, JoinArgs a) {
-  __shared__ float red[12];
+template <typename T, int VPT, int THREADS>
+__global__ __launch_bounds__(THREADS) void vocab_rows(JoinArgs a) {
+  __shared__ float red[THREADS / 64 * 3];
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const Token token = token_of<T>(a, row);
-    const Part p = segment_stats<T, VPT, true, false>(s, row, red);
-    if (threadIdx.x == 0) write_stat(a, row, RowStat{p.m, p.z < kInf ? p.z : __builtin_nanf(""), p.u}, token);
+    const Row<T> z(a.z, a.ld, row, a.wk.V);
+    const RowStat st = HeldRow<T, VPT, THREADS>(z).template stats<true>(z, a.c, red);
+    if (threadIdx.x == 0) write_stat(a, row, st, token);
+    __syncthreads();
   }
 }
 
@@ -934,25 +1018,40 @@ __global__ __launch_bounds__(kThreads) void distill_finish(DistillArgs a) {
   }
 }
 
-// Rows that one workgroup holds: loss, statistics and, with an output, the
-// gradient in one launch, which reads its logits again out of the caches.  Its
-// steps wait for each other: where the rows fill the chip it pays if they are
-// long and the second read counts (loss and gradient of 256 x 16000 bf16 9.6 us
-// instead of 14.4, 1000 x 5000 fp32 14.0 instead of 25.9, 8000 x 16000 139
-// instead of 192, but 8000 x 1300 51 instead of 46; loss alone of 48 x 8000 fp16
-// 5.5 instead of 6.2, of 2000 x 8000 14.4 instead of 12.3).
-template <typename T, int VPT>
-__global__ __launch_bounds__(kThreads) void distill_rows(StatsArgs s, DistillArgs a) {
-  __shared__ float red[12];
+// Rows that one workgroup holds in registers: loss, statistics and, with an
+// output, the gradient in one launch that reads the logits once (4096 x 32768
+// bf16: 116 us instead of 151, 256 x 16000 12 instead of 16).  A row's steps wait
+// for each other, which costs most where a workgroup fills the CU.
+template <typename T, int VPT, int THREADS>
+__global__ __launch_bounds__(THREADS) void distill_rows(DistillArgs a) {
+  constexpr int N = Elem<T>::kN;
+  __shared__ float red[THREADS / 64 * 3];
   __shared__ FinishLds lds;
+  const int tid = threadIdx.x, w = tid >> 6;
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
-    if (threadIdx.x < 64) pick_row<T>(a, row);
-    const Part p = segment_stats<T, VPT, false, false>(s, row, red);   // (ends with a barrier)
-    const RowStat st{p.m, p.z < kInf ? p.z : __builtin_nanf(""), 0.f};
-    if (a.out) write_grad<T, VPT>(a, s.wk, row, 0, [&] { return st; });
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what is replaced has been written
-    __syncthreads();
-    if (threadIdx.x < 64) finish_row<T>(a, row, lds, st, true, [](int32_t) { return true; });
+    const Row<T> z(a.z, a.ld, row, a.V);
+    const HeldRow<T, VPT, THREADS> held(z);
+    if (w == 0) pick_row<T>(a, row);
+    const RowStat st = held.template stats<false>(z, a.c, red);
+    if (a.out) {
+      T* out = static_cast<T*>(a.out) + row * a.ldo;
+      const float wt = (a.weight ? a.weight[row] : 1.f) * a.inv_t, ts = a.stat[row * 4 + 3];
+      const bool zero = wt == 0.f || ts == 0.f;   // nothing flows into the row
+      const float o = origin(st.m), scale = ts != ts ? ts : st.z == 0.f ? 0.f : wt / st.z;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        const int v = j * THREADS + tid;
+        if (v >= z.nv) break;
+        float x[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = zero ? 0.f : exp2_of(Elem<T>::get(held.r[j], i), o, a.c) * scale;
+        stream_vec(out + z.col(v), Elem<T>::pack(x));
+      }
+      if (held.extra >= 0) out[held.extra] = Elem<T>::cast(zero ? 0.f : exp2_of(held.tail, o, a.c) * scale);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what is replaced has been written
+      __syncthreads();
+    }
+    if (w == 0) finish_row<T>(a, row, lds, st, true, [](int32_t) { return true; });
     __syncthreads();
   }
 }
@@ -966,7 +1065,7 @@ struct Plan {
   int vpt;
 };
 Plan plan(int64_t n, int64_t V, int type, int most) {
-  const int64_t pages = (V / (type == kF32 ? 4 : 8) + kThreads - 1) / kThreads;
+  const int64_t pages = pages_of(V, type);
   Plan p;
   p.vpt = most;
   while (p.vpt > 1 && p.vpt / 2 >= pages) p.vpt /= 2;
@@ -987,7 +1086,13 @@ void with_vpt(int vpt, F&& f) {
   f(std::integral_constant<int, MOST>());
 }
 
-constexpr int64_t kFewRows = 1024;   // of distill_rows whatever their length
+// vocab_rows: always for rows of up to 16 pages (256 x 16000 bf16 4.5 us instead
+// of 7.3, 4096 x 32768 49 instead of 56); a workgroup of 16 waves for longer ones
+// fills a CU alone (256 x 65536 9.0 instead of 10.3, 1024 35.9 instead of 25.9).
+bool in_one_launch(int64_t n, int64_t V, int type) {
+  const int64_t pages = pages_of(V, type);
+  return pages <= 16 || (pages <= 32 && n <= 256);
+}
 
 // The gradient's launches: one where its workgroups are on the chip all at once
 constexpr int64_t kFinishGroups = 2048;
@@ -1002,6 +1107,21 @@ void launch_grad(const DistillArgs& a, const Plan& q, hipStream_t s) {
   });
   if (!finish)
     hipLaunchKernelGGL((distill_finish<T, JOIN>), dim3(groups_of((a.n + 3) / 4)), dim3(kThreads), 0, s, a);
+}
+
+// distill_rows, or false where the other launches are better: the loss alone has
+// no second read to save (1024 rows of 8000 bf16 7.4 us instead of 8.6, 2048 12.9
+// instead of 11.9), and a workgroup of 16 waves leaves the chip empty in a short
+// call (128 x 65536 bf16 16.4 us instead of 14.8, 256 17.8 instead of 22.6).
+template <typename T>
+bool launch_rows(const DistillArgs& a, int type, hipStream_t s) {
+  const int64_t pages = pages_of(a.V, type);
+  if (a.out ? pages > (a.n < 256 ? 16 : 32) : pages > 16 || a.n > 1024) return false;
+  with_rows(pages, [&](auto vpt, auto threads) {
+    constexpr int kVpt = decltype(vpt)::value, kRowThreads = decltype(threads)::value;
+    hipLaunchKernelGGL((distill_rows<T, kVpt, kRowThreads>), dim3(groups_of(a.n)), dim3(kRowThreads), 0, s, a);
+  });
+  return true;
 }
 
 // Threads a group whose maximum is kept for the alternatives: as many as leave
@@ -1020,20 +1140,21 @@ int group_lanes(int64_t S, int k) {
 
 }  // namespace
 
-// bytes of workspace of spmm_token_logprobs and (k = 0) of the distillation
+// bytes of workspace of spmm_token_logprobs (k >= 0) and of the distillation (k = -1)
 SPMM_EXPORT int64_t spmm_vocab_ws(int64_t n, int64_t V, int type, int k) {
-  if (!sizes_ok(n, V, type) || k < 0 || k > kMaxTop || k > V) return -1;
+  if (!sizes_ok(n, V, type) || k < -1 || k > kMaxTop || k > V) return -1;
+  if (k == 0 && in_one_launch(n, V, type)) return 0;
   const int64_t S = plan(n, V, type, kStatsPages).wk.S;
-  return n * S * (int64_t)(sizeof(Part) + (k ? kThreads / group_lanes(S, k) * sizeof(uint32_t) : 0));
+  return n * S * (int64_t)(sizeof(Part) + (k > 0 ? kThreads / group_lanes(S, k) * sizeof(uint32_t) : 0));
 }
 
 SPMM_EXPORT int spmm_token_logprobs(const void* z, int64_t ld, int64_t n, int64_t V, int type, const void* tok, int wide,
                                     int k, float c, float inv_t, float* stat, int64_t* rowptr, int32_t* top_col,
                                     float* top_val, void* ws, int64_t ws_bytes, hipStream_t s) {
   const int64_t need = spmm_vocab_ws(n, V, type, k);
-  if (need < 0 || ws_bytes < need) return (int)hipErrorInvalidValue;
+  if (k < 0 || need < 0 || ws_bytes < need) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
-  const Plan p = plan(n, V, type, kStatsPages), whole = plan(kFill, V, type, kStatsPages);
+  const Plan p = plan(n, V, type, kStatsPages);
   const int64_t S = p.wk.S;
   Part* part = static_cast<Part*>(ws);
   uint32_t* keys = reinterpret_cast<uint32_t*>(part + n * S);
@@ -1041,10 +1162,10 @@ SPMM_EXPORT int spmm_token_logprobs(const void* z, int64_t ld, int64_t n, int64_
   const StatsArgs sa{z, ld, n, p.wk, c, part, keys, lanes};
   const JoinArgs ja{z, ld, n, p.wk, p.vpt, c, inv_t, part, tok, wide, k, lanes, keys, stat, rowptr, top_col, top_val};
   SPMM_VOCAB_TYPE(type, T, {
-    if (k == 0 && whole.wk.S == 1) {
-      const StatsArgs ra{z, ld, n, whole.wk, c, nullptr, nullptr, 1};
-      with_vpt<kStatsPages>(whole.vpt, [&](auto e) {
-        hipLaunchKernelGGL((vocab_rows<T, decltype(e)::value>), dim3(groups_of(n)), dim3(kThreads), 0, s, ra, ja);
+    if (k == 0 && in_one_launch(n, V, type)) {
+      with_rows(pages_of(V, type), [&](auto vpt, auto threads) {
+        constexpr int kVpt = decltype(vpt)::value, kRowThreads = decltype(threads)::value;
+        hipLaunchKernelGGL((vocab_rows<T, kVpt, kRowThreads>), dim3(groups_of(n)), dim3(kRowThreads), 0, s, ja);
       });
       SPMM_LAUNCH_CHECK();
       return 0;
@@ -1086,21 +1207,16 @@ SPMM_EXPORT int spmm_distill(const void* z, int64_t ld, int64_t n, int64_t V, in
                              const int32_t* col, const void* val, int val_type, int64_t nnz, float c, float inv_t,
                              float* loss, float* stat, float* picked, const float* weight, void* out, int64_t ldo,
                              void* ws, int64_t ws_bytes, hipStream_t s) {
-  const int64_t need = spmm_vocab_ws(n, V, type, 0);
+  const int64_t need = spmm_vocab_ws(n, V, type, -1);
   if (need < 0 || ws_bytes < need || val_type < 0 || val_type > 2) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
   const Plan p = plan(n, V, type, kStatsPages), q = plan(n, V, type, kGradPages);
   Part* part = static_cast<Part*>(ws);
   const StatsArgs sa{z, ld, n, p.wk, c, part, nullptr, 1};
-  const Plan whole = plan(kFill, V, type, kStatsPages);
   const DistillArgs a{z, ld, n, V, q.wk, c, inv_t, part, p.wk.S, Teacher{rowptr, col, val, val_type, nnz}, loss, stat,
                       picked, weight, out, ldo};
   SPMM_VOCAB_TYPE(type, T, {
-    if (whole.wk.S == 1 && (n <= kFewRows || (out && whole.vpt == kStatsPages))) {
-      const StatsArgs ra{z, ld, n, whole.wk, c, nullptr, nullptr, 1};
-      with_vpt<kStatsPages>(whole.vpt, [&](auto e) {
-        hipLaunchKernelGGL((distill_rows<T, decltype(e)::value>), dim3(groups_of(n)), dim3(kThreads), 0, s, ra, a);
-      });
+    if (launch_rows<T>(a, type, s)) {
       SPMM_LAUNCH_CHECK();
       return 0;
     }

@@ -77,7 +77,7 @@ def _run(logits, teacher, weight, temperature, out, gradient) -> Tuple[DistillLo
     weight = R.per_row(weight, n, "weight")
     inv_t = R.inverse_temperature(temperature)
     gpu = dev.type == "cuda"
-    ws = _native.hip().spmm_vocab_ws(n, V, code, 0) if gpu else 0
+    ws = _native.hip().spmm_vocab_ws(n, V, code, -1) if gpu else 0
     head = (5 * n + nnz + 3) // 4 * 4   # (the workspace starts at 16 bytes)
     saved = torch.empty(head + ws // 4, dtype=torch.float32, device=dev)
     res = DistillLoss(saved[:n], saved, n, nnz, float(temperature))

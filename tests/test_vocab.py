@@ -604,6 +604,16 @@ def test_distill_many_rows(dtype, n, V):
     check_distill(z, T, 1.0, w, "cuda", inplace=True)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_many_long_rows(dtype):
+    """More workgroups than are on the chip at once, rows longer than one of them holds."""
+    z, _ = logits(130, 131100, dtype, seed=41)
+    w = torch.rand(130, generator=gen(42)) + 0.1
+    w[5] = 0.0
+    check_distill(z, random_teacher(130, 131100, 90, seed=43), 1.5, w, "cuda", inplace=True)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_distill_long_teacher_rows(dev):
     """Thousands of entries a row: ascending columns, absent ones behind them, one column twice, any order."""
