@@ -75,14 +75,14 @@ struct Row {
 // first workgroup.
 struct Walk {
   int64_t V, S;   // columns, workgroups a row
-  int step;       // 1 or 8
+  int step_log;   // of 1 or 8 (2: the halves of a workgroup of 512 threads)
   __device__ __forceinline__ int page(int seg, int j, int vpt) const {
-    return step == 1 ? seg * vpt + j : ((seg >> 3) * vpt + j) * 8 + (seg & 7);
+    return (((seg >> step_log) * vpt + j) << step_log) + (seg & ((1 << step_log) - 1));
   }
   // the workgroup that has a vector (-1: an extra element)
   __device__ __forceinline__ int seg_of(int vec, int vpt) const {
-    const int p = vec / 256;
-    return vec < 0 ? 0 : step == 1 ? p / vpt : p / (8 * vpt) * 8 + (p & 7);
+    const int p = vec / 256, in = p & ((1 << step_log) - 1);
+    return vec < 0 ? 0 : (((p >> step_log) / vpt) << step_log) + in;
   }
 };
 
@@ -238,7 +238,7 @@ template <typename T, int VPT, int THREADS>
 struct HeldRow {
   static constexpr int N = Elem<T>::kN, kWaves = THREADS / 64;
   u32x4 r[VPT];
-  float tail;
+  float tail, mx, zs;   // mx, zs: maximum and sum of this thread's elements
   int extra;
   __device__ __forceinline__ explicit HeldRow(const Row<T>& z) {
     const int tid = threadIdx.x;
@@ -252,20 +252,21 @@ struct HeldRow {
   }
   // red: 3 kWaves floats in LDS, which a barrier behind this call separates from their next use.  ENT: U too
   template <bool ENT>
-  __device__ __forceinline__ RowStat stats(const Row<T>& z, float c, float* red) const {
+  __device__ __forceinline__ RowStat stats(const Row<T>& z, float c, float* red) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     typename Elem<T>::Max most;
     most.one(tail);
 #pragma unroll
     for (int j = 0; j < VPT; ++j) most.vec(r[j]);
-    const float wm = wave_max(most.get());
+    mx = most.get();
+    const float wm = wave_max(mx);
     if (lane == 0) red[w] = wm;
     __syncthreads();
     RowStat st{red[0], 0.f, 0.f};
 #pragma unroll
     for (int q = 1; q < kWaves; ++q) st.m = fmaxf(st.m, red[q]);
     const float o = origin(st.m);
-    float zs = 0.f, us = 0.f;
+    float us = 0.f;
     auto sum = [&](auto masked) {
       zs = us = 0.f;
       auto add = [&](float x) {
@@ -285,11 +286,10 @@ struct HeldRow {
     };
     sum(std::false_type());
     if (ENT && __ballot(us != us)) sum(std::true_type());   // (0 times -inf, as in segment_stats)
-    zs = wave_sum(zs);
-    us = ENT ? wave_sum(us) : 0.f;
+    const float zw = wave_sum(zs), uw = ENT ? wave_sum(us) : 0.f;
     if (lane == 0) {
-      red[kWaves + w] = zs;
-      red[2 * kWaves + w] = us;
+      red[kWaves + w] = zw;
+      red[2 * kWaves + w] = uw;
     }
     __syncthreads();
 #pragma unroll
@@ -299,6 +299,18 @@ struct HeldRow {
     }
     st.z = st.z < kInf ? st.z : __builtin_nanf("");
     return st;
+  }
+  // the largest key of this thread's elements, behind stats()
+  __device__ __forceinline__ uint32_t key() const {
+    uint32_t k = key_of(mx);
+    if (!(zs < kInf)) {   // a NaN among them, or +inf
+      k = key_of(tail);
+#pragma unroll
+      for (int j = 0; j < VPT; ++j)
+#pragma unroll
+        for (int i = 0; i < N; ++i) k = max_u(k, key_of(Elem<T>::get(r[j], i)));
+    }
+    return k;
   }
 };
 
@@ -357,7 +369,8 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// The k largest logits of a row, in order, to out[0 .. k), by one wave.
+// The k largest logits of a row, in order, to out[0 .. k), by one wave; keys: its
+// groups' maxima.
 //
 // `from`, a key that at least k elements reach, starts as the k-th largest of
 // the groups' maxima.  The elements that reach it are collected from the groups
@@ -369,7 +382,7 @@ __device__ __forceinline__ int wave_scan(int x) {
 // round trips to memory and into fetching code that no wave has run before: the
 // loops are kept short and not unrolled.
 template <typename T, typename F>
-__device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& s, F&& out) {
+__device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, const uint32_t* keys, TopLds& s, F&& out) {
   constexpr int N = Elem<T>::kN;
   const int lane = threadIdx.x & 63, k = a.k;
   const unsigned long long below = (1ull << lane) - 1ull;
@@ -377,7 +390,6 @@ __device__ __forceinline__ void row_top(const JoinArgs& a, int64_t row, TopLds& 
   // vectors a group, and what else is a power of two, as shifts
   const int lanes_log = __builtin_ctz(a.lanes), slots_log = lanes_log + __builtin_ctz(a.vpt), per_log = 8 - lanes_log;
   const int groups = (int)(a.wk.S << per_log);
-  const uint32_t* keys = a.keys + row * groups;
   const bool in_regs = groups <= 64 * kKeyRegs;
   uint32_t held[kKeyRegs];
 #pragma unroll
@@ -593,15 +605,37 @@ __device__ __forceinline__ void write_stat(const JoinArgs& a, int64_t row, const
   a.stat[3 * a.n + row] = st.z;
 }
 
-// Rows that one workgroup holds, without alternatives: all in one launch.
-template <typename T, int VPT, int THREADS>
+// a row's alternatives, by one wave
+template <typename T>
+__device__ __forceinline__ void write_top(const JoinArgs& a, int64_t row, const RowStat& st, const uint32_t* keys,
+                                          TopLds& s) {
+  if ((threadIdx.x & 63) == 0) {
+    a.rowptr[row] = row * a.k;
+    if (row == a.n - 1) a.rowptr[a.n] = a.n * a.k;
+  }
+  row_top<T>(a, row, keys, s, [&](int place, uint64_t e) {
+    a.top_col[row * a.k + place] = col_of(e);
+    a.top_val[row * a.k + place] = ln_q_of(a, st, value_of((uint32_t)(e >> 32)));
+  });
+}
+
+// Rows that one workgroup holds: all in one launch.  Its groups are its threads.
+template <typename T, int VPT, int THREADS, bool TOP>
 __global__ __launch_bounds__(THREADS) void vocab_rows(JoinArgs a) {
   __shared__ float red[THREADS / 64 * 3];
+  __shared__ uint32_t keys[TOP ? THREADS : 1];
+  __shared__ std::conditional_t<TOP, TopLds, int> top;
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const Token token = token_of<T>(a, row);
     const Row<T> z(a.z, a.ld, row, a.wk.V);
-    const RowStat st = HeldRow<T, VPT, THREADS>(z).template stats<true>(z, a.c, red);
+    HeldRow<T, VPT, THREADS> held(z);
+    const RowStat st = held.template stats<true>(z, a.c, red);
     if (threadIdx.x == 0) write_stat(a, row, st, token);
+    if constexpr (TOP) {
+      keys[threadIdx.x] = held.key();
+      __syncthreads();
+      if (threadIdx.x < 64) write_top<T>(a, row, st, keys, top);
+    }
     __syncthreads();
   }
 }
@@ -615,16 +649,7 @@ __global__ __launch_bounds__(kThreads) void vocab_join(JoinArgs a) {
     const Token token = token_of<T>(a, row);
     const RowStat st = join_parts(a.part + row * a.wk.S, a.wk.S, a.c);
     if (lane == 0) write_stat(a, row, st, token);
-    if constexpr (TOP) {
-      if (lane == 0) {
-        a.rowptr[row] = row * a.k;
-        if (row == a.n - 1) a.rowptr[a.n] = a.n * a.k;
-      }
-      row_top<T>(a, row, top[w], [&](int place, uint64_t e) {
-        a.top_col[row * a.k + place] = col_of(e);
-        a.top_val[row * a.k + place] = ln_q_of(a, st, value_of((uint32_t)(e >> 32)));
-      });
-    }
+    if constexpr (TOP) write_top<T>(a, row, st, a.keys + row * a.wk.S * (kThreads / a.lanes), top[w]);
   }
 }
 
@@ -1030,7 +1055,7 @@ __global__ __launch_bounds__(THREADS) void distill_rows(DistillArgs a) {
   const int tid = threadIdx.x, w = tid >> 6;
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const Row<T> z(a.z, a.ld, row, a.V);
-    const HeldRow<T, VPT, THREADS> held(z);
+    HeldRow<T, VPT, THREADS> held(z);
     if (w == 0) pick_row<T>(a, row);
     const RowStat st = held.template stats<false>(z, a.c, red);
     if (a.out) {
@@ -1071,7 +1096,7 @@ Plan plan(int64_t n, int64_t V, int type, int most) {
   while (p.vpt > 1 && p.vpt / 2 >= pages) p.vpt /= 2;
   for (;; p.vpt /= 2) {
     const int64_t step = pages > p.vpt ? 8 : 1, span = step * p.vpt, S = (pages + span - 1) / span * step;
-    p.wk = Walk{V, S < 1 ? 1 : S, (int)step};
+    p.wk = Walk{V, S < 1 ? 1 : S, step == 8 ? 3 : 0};
     if (p.vpt == 1 || n * p.wk.S >= kFill) return p;
   }
 }
@@ -1086,11 +1111,15 @@ void with_vpt(int vpt, F&& f) {
   f(std::integral_constant<int, MOST>());
 }
 
-// vocab_rows: always for rows of up to 16 pages (256 x 16000 bf16 4.5 us instead
-// of 7.3, 4096 x 32768 49 instead of 56); a workgroup of 16 waves for longer ones
-// fills a CU alone (256 x 65536 9.0 instead of 10.3, 1024 35.9 instead of 25.9).
-bool in_one_launch(int64_t n, int64_t V, int type) {
+// vocab_rows without alternatives: always for rows of up to 16 pages (256 x
+// 16000 bf16 4.5 us instead of 7.3, 4096 x 32768 49 instead of 56); a workgroup
+// of 16 waves for longer ones fills a CU alone (256 x 65536 9.0 instead of 10.3,
+// 1024 35.9 instead of 25.9).  With them it holds its CU while one wave looks for
+// them: for few rows (k = 20, 256 x 32768 bf16 12.6 us instead of 17.8, 1024 x
+// 8000 11.1 instead of 14.4, 1024 x 16000 19.9 instead of 18.0).
+bool in_one_launch(int64_t n, int64_t V, int type, int k) {
   const int64_t pages = pages_of(V, type);
+  if (k > 0) return pages <= 16 && n <= 1024 && n * pages <= 4096;
   return pages <= 16 || (pages <= 32 && n <= 256);
 }
 
@@ -1143,7 +1172,7 @@ int group_lanes(int64_t S, int k) {
 // bytes of workspace of spmm_token_logprobs (k >= 0) and of the distillation (k = -1)
 SPMM_EXPORT int64_t spmm_vocab_ws(int64_t n, int64_t V, int type, int k) {
   if (!sizes_ok(n, V, type) || k < -1 || k > kMaxTop || k > V) return -1;
-  if (k == 0 && in_one_launch(n, V, type)) return 0;
+  if (k >= 0 && in_one_launch(n, V, type, k)) return 0;
   const int64_t S = plan(n, V, type, kStatsPages).wk.S;
   return n * S * (int64_t)(sizeof(Part) + (k > 0 ? kThreads / group_lanes(S, k) * sizeof(uint32_t) : 0));
 }
@@ -1162,10 +1191,20 @@ SPMM_EXPORT int spmm_token_logprobs(const void* z, int64_t ld, int64_t n, int64_
   const StatsArgs sa{z, ld, n, p.wk, c, part, keys, lanes};
   const JoinArgs ja{z, ld, n, p.wk, p.vpt, c, inv_t, part, tok, wide, k, lanes, keys, stat, rowptr, top_col, top_val};
   SPMM_VOCAB_TYPE(type, T, {
-    if (k == 0 && in_one_launch(n, V, type)) {
+    if (in_one_launch(n, V, type, k)) {
       with_rows(pages_of(V, type), [&](auto vpt, auto threads) {
         constexpr int kVpt = decltype(vpt)::value, kRowThreads = decltype(threads)::value;
-        hipLaunchKernelGGL((vocab_rows<T, kVpt, kRowThreads>), dim3(groups_of(n)), dim3(kRowThreads), 0, s, ja);
+        JoinArgs ra = ja;
+        ra.wk = Walk{V, kRowThreads / kThreads, kRowThreads == 512 ? 1 : 0};
+        ra.vpt = kVpt;
+        ra.lanes = 1;
+        if constexpr (kRowThreads <= 512)
+          if (k) {
+            hipLaunchKernelGGL((vocab_rows<T, kVpt, kRowThreads, true>), dim3(groups_of(n)), dim3(kRowThreads), 0, s,
+                               ra);
+            return;
+          }
+        hipLaunchKernelGGL((vocab_rows<T, kVpt, kRowThreads, false>), dim3(groups_of(n)), dim3(kRowThreads), 0, s, ra);
       });
       SPMM_LAUNCH_CHECK();
       return 0;

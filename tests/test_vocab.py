@@ -355,6 +355,21 @@ def test_logprobs_long_rows_of_ties_and_infinities(dev, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V", [(1100, 500), (520, 16387), (300, 33003), (1030, 8199)])
+def test_logprobs_many_rows(dtype, n, V):
+    """More rows than are taken in one launch with their alternatives."""
+    z, tok = logits(n, V, dtype, seed=44)
+    z[:, ::3] = -math.inf
+    z[5] = -math.inf
+    z[6] = 1.0
+    z[7, V // 2], z[8, 3] = math.nan, math.inf
+    tok[::9] = -1
+    check_logprobs(z, tok, 17, 1.3, "cuda")
+    check_logprobs(z, tok, 0, 1.3, "cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 def test_logprobs_rows_of_millions(dtype):
     """More groups in a row than a wave keeps in registers."""
     V = 9_000_001
