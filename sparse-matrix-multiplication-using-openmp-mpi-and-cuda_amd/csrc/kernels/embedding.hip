@@ -370,9 +370,14 @@ struct GradArgs {
   int brief;                // embed_grad_brief, without sorted entries
 };
 
-// Sorted entries a wave sums: 8 in a short batch, which has few waves to hide
-// their loads behind; 32 else, which writes a quarter of the partial rows.
-constexpr int64_t kShortBatch = 2048;
+// Sorted entries a wave sums.  Few waves have little to hide their loads behind:
+// 3000 tokens of 500 columns take 26 us with 8 entries a wave, 31 with 16 and 43
+// with 32; 20548 of 857 53, 53 and 60; 12000 of 4096 87, 81 and 79.  One token
+// only, whose partial rows are joined by one workgroup: 41, 33 and 32 us for 4000
+// of 128 columns, 194, 114 and 77 for 32000 of 256.
+inline int64_t tile_of(int64_t entries) {   // tokens times slices
+  return entries <= 6144 ? 8 : entries <= 65536 ? 16 : 32;
+}
 constexpr int kFlight = 8;   // row loads in flight
 constexpr int64_t kNarrow = 8;   // columns, below which rows are summed by embed_grad_narrow
 constexpr int kFillBytes = 16384, kFillPieces = 8;
@@ -741,6 +746,12 @@ __global__ __launch_bounds__(64 * kBriefWaves) void embed_grad_brief(GradArgs a,
   if (w == 0 && c < a.D) finish_row<TO, N>(a, key, c, from, acc);
 }
 
+// slices of a row of dY, 64 lanes' vectors each
+int64_t lane_slices(int64_t D, int in_type) {
+  const int64_t columns = 64 * (in_type == kF32 ? 4 : 8);
+  return (D + columns - 1) / columns;
+}
+
 struct GradSizes {
   int64_t tile, tiles, sort_tiles, keys, cnt, slots, total;
   int bits, passes, rounds;
@@ -748,13 +759,13 @@ struct GradSizes {
 
 // Layout of the workspace: sorted keys and positions, slots, the same two again
 // and digit counters for the radix passes, partial rows.
-bool grad_sizes(int64_t n, int64_t V, int64_t D, GradSizes& g) {
+bool grad_sizes(int64_t n, int64_t V, int64_t D, int in_type, GradSizes& g) {
   if (n < 0 || n >= (1ll << 31) - (1 << 20) || V < 1 || V >= (1ll << 31) - 1 || D < 1) return false;
   int total_bits = 1;
   while ((V >> total_bits) != 0) ++total_bits;   // keys 0 .. V
   g.passes = (total_bits + kMaxBits - 1) / kMaxBits;
   g.bits = (total_bits + g.passes - 1) / g.passes;
-  g.tile = n <= kShortBatch ? 8 : 32;
+  g.tile = tile_of(n * lane_slices(D, in_type));
   g.tiles = (n + g.tile - 1) / g.tile;
   g.rounds = n <= kFewTiles * 256 * kSmallRounds ? kSmallRounds : kLargeRounds;
   g.sort_tiles = (n + 256 * g.rounds - 1) / (256 * g.rounds);
@@ -766,11 +777,6 @@ bool grad_sizes(int64_t n, int64_t V, int64_t D, GradSizes& g) {
   return true;
 }
 
-// slices of a row of dY, 64 lanes' vectors each
-int64_t lane_slices(int64_t D, int in_type) {
-  const int64_t columns = 64 * (in_type == kF32 ? 4 : 8);
-  return (D + columns - 1) / columns;
-}
 bool is_brief(int64_t n, int64_t D, int in_type, int64_t ldw, int accumulate) {
   return n <= kBriefTokens && n * lane_slices(D, in_type) <= kBriefGroups && D >= kNarrow && (accumulate || ldw == D);
 }
@@ -824,7 +830,7 @@ SPMM_EXPORT int spmm_embedding(const void* W, int64_t ldw, int64_t V, int64_t D,
 // bytes of workspace, or -1 for sizes that the kernels do not take; ldw: row stride of the table
 SPMM_EXPORT int64_t spmm_embedding_grad_ws(int64_t n, int64_t V, int64_t D, int in_type, int64_t ldw, int accumulate) {
   GradSizes g;
-  if (!grad_sizes(n, V, D, g)) return -1;
+  if (!grad_sizes(n, V, D, in_type, g)) return -1;
   return is_brief(n, D, in_type, ldw, accumulate) ? 0 : g.total;
 }
 
@@ -832,7 +838,7 @@ SPMM_EXPORT int spmm_embedding_grad(const void* dy, int64_t lddy, int in_type, c
                                     int64_t V, int64_t D, float scale, void* dw, int64_t ldw, int out_type,
                                     int accumulate, void* ws, int64_t ws_bytes, hipStream_t s) {
   GradSizes g;
-  if (!grad_sizes(n, V, D, g)) return (int)hipErrorInvalidValue;
+  if (!grad_sizes(n, V, D, in_type, g)) return (int)hipErrorInvalidValue;
   const bool brief = is_brief(n, D, in_type, ldw, accumulate);
   if (!brief && ws_bytes < g.total) return (int)hipErrorInvalidValue;
   uint32_t* ka = static_cast<uint32_t*>(ws);   // (all null in a brief call, which uses none of it)
