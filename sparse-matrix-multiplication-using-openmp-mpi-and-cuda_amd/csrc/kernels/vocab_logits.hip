@@ -89,6 +89,7 @@ struct Walk {
 // the point that the u_j of a row are measured from
 __device__ __forceinline__ float origin(float m) { return m == -kInf ? 0.f : m; }
 
+// (the instruction's results below 2^-126 are zero)
 __device__ __forceinline__ float exp2_of(float z, float m, float c) { return __builtin_amdgcn_exp2f((z - m) * c); }
 __device__ __forceinline__ float log2_of(float z) { return z == 0.f ? 0.f : __builtin_amdgcn_logf(z); }
 
