@@ -179,9 +179,6 @@ __device__ __forceinline__ float wave_sum(float x) {
     return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
   }));
 }
-__device__ __forceinline__ int wave_sum_i(int x) {
-  return (int)over_wave((uint32_t)x, [](uint32_t a, uint32_t b) { return a + b; });
-}
 
 // max(a, b, c) as one instruction, without the quieting of signalling NaNs that
 // fmaxf asks for: such a NaN makes the result a NaN, which the next maximum
