@@ -990,7 +990,7 @@ __device__ __forceinline__ bool write_grad(const DistillArgs& a, const Walk& wk,
 // their segments'.
 //
 // Bytes bound a step of loss and gradient: the logits are read twice and the
-// gradient written once, 3.2 GB for 4096 x 131072 bf16 in 497 us (521 at the
+// gradient written once, 3.2 GB for 4096 x 131072 bf16 in 500 us (521 at the
 // rate of a large copy).  One read would take a row of 256 KB in registers
 // from its statistics to its gradient, half of a CU's: a workgroup a row with
 // half of it kept took 574 us, with all of it spilling 670, where these kernels
@@ -998,9 +998,10 @@ __device__ __forceinline__ bool write_grad(const DistillArgs& a, const Walk& wk,
 // gradient of 128 MB at a time) is no faster than one from memory: 660 us.
 //
 // FINISH: few workgroups, where a launch costs more than it does: each one ends
-// its own columns of the row itself, the first one the loss (48 x 32768 fp16, 32
-// entries: 8.4 us instead of 10.3, from the host 19.6 instead of 22.1; 1000 x
-// 32768, 8000 workgroups: 52.8 instead of 47.5).
+// its own columns of the row itself, the first one the loss (128 x 131072 bf16
+// 21.6 us instead of 22.9 and a launch less for the host, the gradient alone of
+// 48 x 32768 fp16 4.3 instead of 5.8; 1000 x 32768, 8000 workgroups, took 52.8
+// instead of 47.5).
 template <typename T, int VPT, bool JOIN, bool FINISH>
 __global__ __launch_bounds__(kThreads) void distill_grad(DistillArgs a) {
   __shared__ std::conditional_t<FINISH, FinishLds, int> lds;
@@ -1009,17 +1010,16 @@ __global__ __launch_bounds__(kThreads) void distill_grad(DistillArgs a) {
   for (int64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
     const int64_t row = t / wk.S;
     const int seg = (int)(t - row * wk.S);
-    RowStat st;
     auto stat = [&] {
-      if (JOIN) st = join_parts(a.part + row * a.S, a.S, a.c);
-      else st = RowStat{a.stat[row * 4], a.stat[row * 4 + 1], 0.f};
-      return st;
+      return JOIN ? join_parts(a.part + row * a.S, a.S, a.c) : RowStat{a.stat[row * 4], a.stat[row * 4 + 1], 0.f};
     };
-    const bool flows = write_grad<T, VPT>(a, wk, row, seg, stat);
-    if constexpr (FINISH) {
-      if (!flows) {
+    if constexpr (!FINISH) {
+      write_grad<T, VPT>(a, wk, row, seg, stat);
+    } else {
+      RowStat st;
+      if (!write_grad<T, VPT>(a, wk, row, seg, [&] { return st = stat(); })) {
         if (!JOIN || seg != 0) continue;   // (the loss is still to be written)
-        stat();
+        st = stat();
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what is replaced has been written
       __syncthreads();
