@@ -137,13 +137,23 @@ def check(rc: int, what: str) -> None:
         raise RuntimeError(f"{what} failed with HIP error {rc}")
 
 
+def null(t) -> int:
+    """The pointer of a tensor whose ``data_ptr()`` is 0: an empty one's.  One
+    with elements has no memory (a meta, fake or zero tensor, a subclass that
+    wraps others), which a native call would read through a null pointer."""
+    if t.numel():
+        raise ValueError(f"a {type(t).__name__} of shape {tuple(t.shape)} on {t.device} has no memory of its own, "
+                         "which native code reads")
+    return 0
+
+
 def ptr(t) -> int:
     """Raw data pointer of a torch tensor / numpy array (0 for empty; None,
     i.e. a null pointer, for None)."""
     if t is None:
         return None
     if hasattr(t, "data_ptr"):
-        return t.data_ptr()
+        return t.data_ptr() or null(t)
     return t.ctypes.data
 
 

@@ -31,7 +31,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
-from .._native import c_vp
+from .._native import c_vp, null
 from . import rows as R
 from .csr import CSR
 from .logprobs import LOG2E, gradient_out, logits_rows
@@ -76,7 +76,7 @@ def _run(logits, teacher, weight, temperature, out, gradient) -> Tuple[DistillLo
     R.same_device(dev, weight=weight)
     weight = R.per_row(weight, n, "weight")
     inv_t = R.inverse_temperature(temperature)
-    gpu = dev.type == "cuda"
+    gpu = R.on_gpu(z)
     ws = _native.hip().spmm_vocab_ws(n, V, code, -1) if gpu else 0
     head = (5 * n + nnz + 3) // 4 * 4   # (the workspace starts at 16 bytes)
     saved = torch.empty(head + ws // 4, dtype=torch.float32, device=dev)
@@ -85,22 +85,24 @@ def _run(logits, teacher, weight, temperature, out, gradient) -> Tuple[DistillLo
         out = gradient_out(out, z)
     if n == 0:
         return res, out
-    at = saved.data_ptr()
-    w = weight.data_ptr() if weight is not None else None
+    at, at_z, at_ptr = saved.data_ptr() or null(saved), z.data_ptr() or null(z), ptr.data_ptr() or null(ptr)
+    at_col, at_val = col.data_ptr() or null(col), val.data_ptr() or null(val)
+    w = weight.data_ptr() or null(weight) if weight is not None else None
+    at_out = out.data_ptr() or null(out) if gradient else None
     if not gpu:
         zf, vf = z.float().contiguous(), val.float()
         acc = torch.empty((n, V), dtype=torch.float32) if gradient else None
         _native.check(_native.host().spmm_cpu_distill(
-            n, V, zf.data_ptr(), ptr.data_ptr(), col.data_ptr(), vf.data_ptr(), nnz, inv_t, at, at + 4 * n, w,
-            acc.data_ptr() if gradient else None, 0), "cpu_distill")
+            n, V, _native.ptr(zf), at_ptr, at_col, _native.ptr(vf), nnz, inv_t, at, at + 4 * n, w, _native.ptr(acc), 0),
+            "cpu_distill")
         if gradient:
             out.copy_(acc)
         return res, out
     with R.on(dev):
         _native.check(_native.hip().spmm_distill(
-            z.data_ptr(), z.stride(0), n, V, code, ptr.data_ptr(), col.data_ptr(), val.data_ptr(), R.TYPES[val.dtype],
-            nnz, LOG2E * inv_t, inv_t, at, at + 4 * n, at + 20 * n, w, out.data_ptr() if gradient else None,
-            out.stride(0) if gradient else 0, at + 4 * head, ws, _native.stream_ptr(dev)), "distill")
+            at_z, z.stride(0), n, V, code, at_ptr, at_col, at_val, R.TYPES[val.dtype], nnz, LOG2E * inv_t, inv_t, at,
+            at + 4 * n, at + 20 * n, w, at_out, out.stride(0) if gradient else 0, at + 4 * head, ws,
+            _native.stream_ptr(dev)), "distill")
     return res, out
 
 
@@ -135,13 +137,13 @@ def distill_grad(logits: torch.Tensor, teacher: CSR, stats: DistillLoss, weight:
     out = gradient_out(out, z)
     if n == 0:
         return out
-    if dev.type != "cuda":
+    if not R.on_gpu(z):
         return _run(z, teacher, weight, stats.temperature, out, True)[1]
-    at = stats.saved.data_ptr()
+    at, at_z, at_ptr = stats.saved.data_ptr() or null(stats.saved), z.data_ptr() or null(z), ptr.data_ptr() or null(ptr)
+    at_col, at_val, at_out = col.data_ptr() or null(col), val.data_ptr() or null(val), out.data_ptr() or null(out)
+    w = weight.data_ptr() or null(weight) if weight is not None else None
     with R.on(dev):
         _native.check(_native.hip().spmm_distill_grad(
-            z.data_ptr(), z.stride(0), n, V, R.TYPES[z.dtype], ptr.data_ptr(), col.data_ptr(), val.data_ptr(),
-            R.TYPES[val.dtype], nnz, LOG2E * inv_t, inv_t, at + 4 * n, at + 20 * n,
-            weight.data_ptr() if weight is not None else None, out.data_ptr(), out.stride(0),
-            _native.stream_ptr(dev)), "distill_grad")
+            at_z, z.stride(0), n, V, R.TYPES[z.dtype], at_ptr, at_col, at_val, R.TYPES[val.dtype], nnz, LOG2E * inv_t,
+            inv_t, at + 4 * n, at + 20 * n, w, at_out, out.stride(0), _native.stream_ptr(dev)), "distill_grad")
     return out

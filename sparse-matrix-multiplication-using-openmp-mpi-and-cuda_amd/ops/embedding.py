@@ -24,7 +24,7 @@ from typing import Optional
 import torch
 
 from .. import _native
-from .._native import c_vp
+from .._native import c_vp, null
 from . import rows as R
 
 _native.register_hip("spmm_embedding", c_vp, C.c_int64, C.c_int64, C.c_int64, C.c_int, c_vp, C.c_int, C.c_int64,
@@ -53,6 +53,7 @@ def embedding(W: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
     W = R.matrix(W, "W")
     dev = W.device
     R.same_device(dev, tokens=tokens)
+    gpu = R.on_gpu(W)
     tok = R.token_ids(tokens)
     scale = _scale(scale)
     V, D = W.shape
@@ -66,7 +67,8 @@ def embedding(W: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
     if n == 0 or D == 0:
         return out
     y = out if out.dim() == 2 else out.view(n, D)
-    if dev.type != "cuda":
+    at_w, at_tok, at_y = W.data_ptr() or null(W), tok.data_ptr() or null(tok), y.data_ptr() or null(y)
+    if not gpu:
         w, t = W.float().contiguous(), tok.to(torch.int64)
         acc = torch.empty((n, D), dtype=torch.float32)
         _native.check(_native.host().spmm_cpu_embedding(n, V, D, _native.ptr(w), _native.ptr(t), scale,
@@ -74,8 +76,8 @@ def embedding(W: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
         y.copy_(acc)
         return out
     with R.on(dev):
-        _native.check(_native.hip().spmm_embedding(W.data_ptr(), W.stride(0), V, D, R.TYPES[W.dtype], tok.data_ptr(),
-                                                   tok.dtype == torch.int64, n, scale, y.data_ptr(), y.stride(0),
+        _native.check(_native.hip().spmm_embedding(at_w, W.stride(0), V, D, R.TYPES[W.dtype], at_tok,
+                                                   tok.dtype == torch.int64, n, scale, at_y, y.stride(0),
                                                    _native.stream_ptr(dev)), "embedding")
     return out
 
@@ -99,6 +101,7 @@ def embedding_grad(dY: torch.Tensor, tokens: torch.Tensor, V: int, scale: float 
     D, n = dY.shape[-1], tokens.numel()
     dev = dY.device
     R.same_device(dev, tokens=tokens)
+    gpu = R.on_gpu(dY)
     dy = R.matrix(dY if dY.dim() == 2 else dY.reshape(n, D), "dY")
     tok = R.token_ids(tokens)
     scale = _scale(scale)
@@ -115,7 +118,8 @@ def embedding_grad(dY: torch.Tensor, tokens: torch.Tensor, V: int, scale: float 
         R.apart(out, dy, "dY", in_place=False)
     if D == 0:
         return out
-    if dev.type != "cuda":
+    at_dy, at_tok, at_out = dy.data_ptr() or null(dy), tok.data_ptr() or null(tok), out.data_ptr() or null(out)
+    if not gpu:
         g, t = dy.float().contiguous(), tok.to(torch.int64)
         acc = out.float().contiguous().clone() if accumulate else torch.zeros((V, D), dtype=torch.float32)
         _native.check(_native.host().spmm_cpu_embedding_grad(n, V, D, _native.ptr(g), _native.ptr(t), scale,
@@ -128,8 +132,8 @@ def embedding_grad(dY: torch.Tensor, tokens: torch.Tensor, V: int, scale: float 
         raise ValueError(f"embedding_grad does not take {n} tokens over {V} rows")
     with R.on(dev):
         ws = torch.empty(bytes_, dtype=torch.uint8, device=dev) if bytes_ else None
-        _native.check(lib.spmm_embedding_grad(dy.data_ptr(), dy.stride(0), R.TYPES[dy.dtype], tok.data_ptr(),
-                                              tok.dtype == torch.int64, n, V, D, scale, out.data_ptr(), out.stride(0),
-                                              R.TYPES[dtype], accumulate, ws.data_ptr() if bytes_ else None, bytes_,
-                                              _native.stream_ptr(dev)), "embedding_grad")
+        _native.check(lib.spmm_embedding_grad(at_dy, dy.stride(0), R.TYPES[dy.dtype], at_tok, tok.dtype == torch.int64,
+                                              n, V, D, scale, at_out, out.stride(0), R.TYPES[dtype], accumulate,
+                                              ws.data_ptr() if bytes_ else None, bytes_, _native.stream_ptr(dev)),
+                      "embedding_grad")
     return out

@@ -28,7 +28,7 @@ from typing import Optional
 import torch
 
 from .. import _native
-from .._native import c_vp
+from .._native import c_vp, null
 from . import rows as R
 from .csr import CSR
 
@@ -85,7 +85,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     k = int(k)
     if not 0 <= k <= min(MAX_TOP, V):
         raise ValueError(f"k must be between 0 and {min(MAX_TOP, V)}, got {k}")
-    gpu = dev.type == "cuda" and n > 0
+    on_gpu = R.on_gpu(z)
+    gpu = on_gpu and n > 0
     bytes_ = _native.hip().spmm_vocab_ws(n, V, R.TYPES[z.dtype], k) if gpu else 0
     kept = bytes_ <= KEPT   # (a row's workspace is whole floats, and starts at 16 bytes)
     stat = torch.empty(4 + (bytes_ // (4 * n) if gpu and kept else 0), n, dtype=torch.float32, device=dev)
@@ -97,22 +98,22 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
                   torch.empty(n * k, dtype=torch.float32, device=dev))
         if n == 0:
             top.rowptr.zero_()
-        elif dev.type != "cuda":
+        elif not on_gpu:
             torch.arange(0, n * k + 1, k, out=top.rowptr)
     res = TokenLogprobs(logprob, entropy, stat, float(temperature), top)
     if n == 0:
         return res
+    at_z, at_tok, at_stat = z.data_ptr() or null(z), tok.data_ptr() or null(tok), stat.data_ptr() or null(stat)
     at = (top.rowptr.data_ptr(), top.col.data_ptr(), top.val.data_ptr()) if k else (None, None, None)
-    if dev.type != "cuda":
+    if not on_gpu:
         zf, t = z.float().contiguous(), tok.to(torch.int64)
-        _native.check(_native.host().spmm_cpu_token_logprobs(n, V, zf.data_ptr(), t.data_ptr(), inv_t, k,
-                                                             stat.data_ptr(), at[1], at[2], 0), "cpu_token_logprobs")
+        _native.check(_native.host().spmm_cpu_token_logprobs(n, V, _native.ptr(zf), _native.ptr(t), inv_t, k, at_stat,
+                                                             at[1], at[2], 0), "cpu_token_logprobs")
         return res
     with R.on(dev):
-        at_stat = stat.data_ptr()
         ws = None if kept else torch.empty(bytes_, dtype=torch.uint8, device=dev)
         _native.check(_native.hip().spmm_token_logprobs(
-            z.data_ptr(), z.stride(0), n, V, R.TYPES[z.dtype], tok.data_ptr(), tok.dtype == torch.int64, k,
+            at_z, z.stride(0), n, V, R.TYPES[z.dtype], at_tok, tok.dtype == torch.int64, k,
             LOG2E * inv_t, inv_t, at_stat, *at, at_stat + 16 * n if kept else ws.data_ptr(), bytes_,
             _native.stream_ptr(dev)), "token_logprobs")
     return res
@@ -129,6 +130,7 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: Token
     logits are not read."""
     R.no_grad_of("token_logprobs_grad", logits, g_logprob, g_entropy, out)
     z = logits_rows(logits)
+    gpu = R.on_gpu(z)
     n, V = z.shape
     dev = z.device
     R.same_device(dev, tokens=tokens, g_logprob=g_logprob, g_entropy=g_entropy, stats=stats.stat)
@@ -147,19 +149,20 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: Token
     out = gradient_out(out, z)
     if n == 0:
         return out
-    at_g = g.data_ptr() if g is not None else None
-    at_h = h.data_ptr() if h is not None else None
-    if dev.type != "cuda":
+    at_z, at_tok, at_stat = z.data_ptr() or null(z), tok.data_ptr() or null(tok), stat.data_ptr() or null(stat)
+    at_out = out.data_ptr() or null(out)
+    at_g = g.data_ptr() or null(g) if g is not None else None
+    at_h = h.data_ptr() or null(h) if h is not None else None
+    if not gpu:
         zf, t = z.float().contiguous(), tok.to(torch.int64)
         acc = torch.empty((n, V), dtype=torch.float32)
-        _native.check(_native.host().spmm_cpu_token_logprobs_grad(n, V, zf.data_ptr(), t.data_ptr(), inv_t,
-                                                                  stat.data_ptr(), at_g, at_h, acc.data_ptr(), 0),
+        _native.check(_native.host().spmm_cpu_token_logprobs_grad(n, V, _native.ptr(zf), _native.ptr(t), inv_t,
+                                                                  at_stat, at_g, at_h, _native.ptr(acc), 0),
                       "cpu_token_logprobs_grad")
         out.copy_(acc)
         return out
     with R.on(dev):
         _native.check(_native.hip().spmm_token_logprobs_grad(
-            z.data_ptr(), z.stride(0), n, V, R.TYPES[z.dtype], tok.data_ptr(), tok.dtype == torch.int64, LOG2E * inv_t,
-            inv_t, stat.data_ptr(), at_g, at_h, out.data_ptr(), out.stride(0), _native.stream_ptr(dev)),
-            "token_logprobs_grad")
+            at_z, z.stride(0), n, V, R.TYPES[z.dtype], at_tok, tok.dtype == torch.int64, LOG2E * inv_t, inv_t, at_stat,
+            at_g, at_h, at_out, out.stride(0), _native.stream_ptr(dev)), "token_logprobs_grad")
     return out

@@ -40,6 +40,15 @@ def same_device(device: torch.device, **others) -> None:
             raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
 
 
+def on_gpu(x: torch.Tensor) -> bool:
+    """Whether x's operators run on the GPU, as opposed to the CPU: there are no others."""
+    if x.is_cuda:
+        return True
+    if not x.is_cpu:
+        raise ValueError(f"operands must be on the CPU or a GPU, got {x.device}")
+    return False
+
+
 def token_ids(tokens: torch.Tensor) -> torch.Tensor:
     if tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"tokens must be int32 or int64, got {tokens.dtype}")

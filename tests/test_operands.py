@@ -1,0 +1,116 @@
+"""What the operators on rows over a vocabulary, and the products beside them,
+refuse because a native call would go wrong on it without a word, and calls of
+theirs that take a path of their own."""
+import math
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import spmm_amd  # noqa: F401
+from spmm_amd.ops.csr import CSR
+from spmm_amd.ops.distill import distill_grad, distill_loss, distill_loss_grad
+from spmm_amd.ops.embedding import embedding, embedding_grad
+from spmm_amd.ops.logprobs import token_logprobs, token_logprobs_grad
+from spmm_amd.ops.spmm import spmm
+
+DEVICES = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+class Operands:
+    """Small operands of all entry points, and each of these as a call of some of them."""
+
+    def __init__(self, dev, dtype=torch.float32):
+        g = torch.Generator().manual_seed(3)
+        self.W = torch.randn(7, 9, generator=g).to(dtype).to(dev)
+        self.dY = torch.randn(3, 9, generator=g).to(dtype).to(dev)
+        self.z = torch.randn(3, 7, generator=g).to(dtype).to(dev)
+        self.tok = torch.tensor([1, 6, 0], device=dev)
+        self.g = torch.randn(3, generator=g).to(dev)
+        self.w = torch.rand(3, generator=g).to(dev)
+        self.T = CSR(3, 7, torch.tensor([0, 2, 2, 5], device=dev),
+                     torch.tensor([1, 4, 0, 3, 6], dtype=torch.int32, device=dev),
+                     torch.randn(5, generator=g).to(dev))
+
+    def change(self, f):
+        """The same with f applied to every floating-point operand."""
+        o = object.__new__(Operands)
+        o.tok = self.tok
+        for name in ("W", "dY", "z", "g", "w"):
+            setattr(o, name, f(getattr(self, name)))
+        o.T = self.T.with_values(f(self.T.val))
+        return o
+
+
+CALLS = {
+    "embedding": lambda o: embedding(o.W, o.tok, scale=1.5),
+    "embedding_grad": lambda o: embedding_grad(o.dY, o.tok, 7, scale=1.5),
+    "token_logprobs": lambda o: token_logprobs(o.z, o.tok, k=2),
+    "token_logprobs_grad": lambda o: token_logprobs_grad(o.z, o.tok, token_logprobs(o.z, o.tok), o.g, o.w),
+    "distill_loss": lambda o: distill_loss(o.z, o.T),
+    "distill_loss_grad": lambda o: distill_loss_grad(o.z, o.T, o.w),
+    "distill_grad": lambda o: distill_grad(o.z, o.T, distill_loss(o.z, o.T), o.w),
+}
+
+
+# ---- tensors without memory of their own ----------------------------------------------------------------------------
+
+class Wrapper(torch.Tensor):
+    """A subclass that holds another tensor and no memory itself."""
+
+    @staticmethod
+    def __new__(cls, x):
+        r = torch.Tensor._make_wrapper_subclass(cls, x.shape, dtype=x.dtype, device=x.device, strides=x.stride())
+        r.inner = x
+        return r
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        out = func(*[a.inner if isinstance(a, Wrapper) else a for a in args], **(kwargs or {}))
+        return Wrapper(out) if isinstance(out, torch.Tensor) else out
+
+
+MEMORYLESS = {
+    "meta": lambda x: x.to("meta"),
+    "fake": lambda x: FakeTensorMode().from_tensor(x),
+    "zero": lambda x: torch._efficientzerotensor(x.shape, dtype=x.dtype, device=x.device),
+    "wrapper": Wrapper,
+}
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", MEMORYLESS)
+@pytest.mark.parametrize("name", CALLS)
+def test_tensors_without_memory_are_refused(dev, kind, name):
+    o = Operands(dev).change(MEMORYLESS[kind])
+    with pytest.raises(ValueError, match="no memory|on the CPU or a GPU|is on"):
+        CALLS[name](o)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", MEMORYLESS)
+def test_single_operands_without_memory_are_refused(dev, kind):
+    f, o = MEMORYLESS[kind], Operands(dev)
+    r, s = token_logprobs(o.z, o.tok), distill_loss(o.z, o.T)
+    T = [CSR(3, 7, f(o.T.rowptr), o.T.col, o.T.val), CSR(3, 7, o.T.rowptr, f(o.T.col), o.T.val),
+         CSR(3, 7, o.T.rowptr, o.T.col, f(o.T.val))]
+    calls = [lambda: embedding(o.W, f(o.tok)), lambda: embedding(o.W, o.tok, out=f(o.dY)),
+             lambda: embedding_grad(o.dY, f(o.tok), 7), lambda: embedding_grad(o.dY, o.tok, 7, out=f(o.W)),
+             lambda: token_logprobs(o.z, f(o.tok)), lambda: token_logprobs_grad(o.z, o.tok, r, f(o.g)),
+             lambda: token_logprobs_grad(o.z, o.tok, r, None, f(o.g)),
+             lambda: token_logprobs_grad(o.z, o.tok, r, o.g, out=f(o.z)),
+             lambda: distill_loss_grad(o.z, o.T, weight=f(o.w)), lambda: distill_loss_grad(o.z, o.T, out=f(o.z)),
+             lambda: distill_grad(o.z, o.T, s, weight=f(o.w))]
+    calls += [lambda t=t: distill_loss(o.z, t) for t in T]
+    for call in calls:
+        with pytest.raises(ValueError, match="no memory|is on|overlap"):
+            call()
+
+
+@pytest.mark.parametrize("kind", MEMORYLESS)
+def test_products_of_tensors_without_memory_are_refused(kind):
+    f, o = MEMORYLESS[kind], Operands("cpu")
+    X = torch.randn(7, 128)
+    for A, x in ((o.T.with_values(f(o.T.val)), X), (CSR(3, 7, f(o.T.rowptr), o.T.col, o.T.val), X), (o.T, f(X))):
+        with pytest.raises(ValueError, match="no memory"):
+            spmm(A, x)
