@@ -4,18 +4,38 @@ from __future__ import annotations
 
 import contextlib
 import math
+import sys
 from typing import Optional
 
 import torch
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # vocab_common.hpp kF32, kBF16, kF16
 _NOTHING = contextlib.nullcontext()
+_tracing = torch._C._get_tracing_state
+_modes = torch._C._len_torch_dispatch_stack
+_functions = torch._C._len_torch_function_stack
+_RECORDING = (torch._C._TorchDispatchModeKey.FAKE, torch._C._TorchDispatchModeKey.FUNCTIONAL)
+
+
+def _traced() -> bool:
+    """Whether torch.jit.trace, make_fx or a fake mode records the calls made
+    here (other modes, such as a default device or a counter of operations, do not)."""
+    if _tracing() is not None:
+        return True
+    proxy = sys.modules.get("torch.fx.experimental.proxy_tensor")   # (its import takes long, and make_fx is in it)
+    if proxy is not None and proxy.get_proxy_mode() is not None:
+        return True
+    return _modes() > 0 and any(torch._C._get_dispatch_mode(k) is not None for k in _RECORDING)
 
 
 def no_grad_of(grad_name: str, *tensors) -> None:
     """These operators are not recorded by autograd; their gradients are
     functions of their own.  A tensor that autograd follows is refused rather
-    than dropped out of its graph without a word."""
+    than dropped out of its graph without a word, and so is a call that a
+    tracer records: it would see the output's allocation and no kernel."""
+    if (_tracing() is not None or _modes() or _functions()) and _traced():
+        raise ValueError("a tracer does not see what this operator computes: call it outside of torch.jit.trace, "
+                         "make_fx and fake tensor modes")
     for t in tensors:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"autograd does not follow this operator: call it under torch.no_grad() or on a detached "

@@ -6,6 +6,8 @@ import math
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils.flop_counter import FlopCounterMode
 
 import spmm_amd  # noqa: F401
 from spmm_amd.ops.csr import CSR
@@ -114,3 +116,53 @@ def test_products_of_tensors_without_memory_are_refused(kind):
     for A, x in ((o.T.with_values(f(o.T.val)), X), (CSR(3, 7, f(o.T.rowptr), o.T.col, o.T.val), X), (o.T, f(X))):
         with pytest.raises(ValueError, match="no memory"):
             spmm(A, x)
+
+
+# ---- tracers --------------------------------------------------------------------------------------------------------
+
+def traced(how, f, x):
+    if how == "jit":
+        return torch.jit.trace(f, (x,), check_trace=False)
+    if how == "fake mode":
+        with FakeTensorMode(allow_non_fake_inputs=True):
+            return f(x)
+    kwargs = {"make_fx": {}, "fake": {"tracing_mode": "fake"}, "symbolic": {"tracing_mode": "symbolic"},
+              "pre-dispatch": {"pre_dispatch": True}}[how]
+    return make_fx(f, **kwargs)(x)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("how", ["jit", "make_fx", "fake", "symbolic", "pre-dispatch", "fake mode"])
+@pytest.mark.parametrize("name", CALLS)
+def test_tracers_are_refused(dev, how, name):
+    """They record the allocation of the output and nothing of the kernel: what they return gives garbage."""
+    o = Operands(dev)
+
+    def call(z):
+        r = CALLS[name](o.change(lambda x: z if x is o.z else x))
+        r = r[1] if isinstance(r, tuple) else r
+        return r if isinstance(r, torch.Tensor) else r.logprob if name == "token_logprobs" else r.loss
+
+    with pytest.raises(ValueError, match="tracer"):
+        traced(how, call, o.z)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_modes_that_record_nothing_are_taken(dev):
+    o = Operands(dev)
+    want = token_logprobs(o.z, o.tok).logprob
+    with torch.device(dev), FlopCounterMode(display=False), torch.inference_mode():
+        assert torch.equal(token_logprobs(o.z, o.tok).logprob, want)
+    assert torch.equal(token_logprobs(o.z, o.tok).logprob, want)
+
+
+def test_compiled_callers_run_the_operators():
+    """torch.compile leaves a caller's compiled parts at these calls and runs them as they are."""
+    o = Operands("cpu")
+
+    def step(z, tok):
+        return token_logprobs(z + 1.0, tok).logprob * 2.0
+
+    f = torch.compile(step, backend="eager")
+    for z in (o.z, o.z * 3.0):
+        assert torch.equal(f(z, o.tok), step(z, o.tok))
