@@ -126,7 +126,7 @@ def distill_grad(logits: torch.Tensor, teacher: CSR, stats: DistillLoss, weight:
     """The gradient alone, where the rows' weights are known only after the
     loss: ``stats`` is what :func:`distill_loss` returned for the same logits
     and teacher.  ``out`` may be the logits themselves."""
-    R.no_grad_of("distill_grad", logits, weight, out, teacher.val)
+    R.no_grad_of("distill_grad", logits, stats.saved, weight, out, teacher.val)
     z, n, V, ptr, col, val = _operands(logits, teacher)
     dev, nnz = z.device, col.shape[0]
     R.same_device(dev, weight=weight, stats=stats.saved)

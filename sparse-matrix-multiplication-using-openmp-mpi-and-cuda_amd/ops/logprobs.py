@@ -128,7 +128,7 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: Token
     same logits and tokens.  ``out`` may be the logits themselves.  A row with
     neither a log-probability's nor an entropy's gradient is zero and its
     logits are not read."""
-    R.no_grad_of("token_logprobs_grad", logits, g_logprob, g_entropy, out)
+    R.no_grad_of("token_logprobs_grad", logits, stats.stat, g_logprob, g_entropy, out)
     z = logits_rows(logits)
     gpu = R.on_gpu(z)
     n, V = z.shape

@@ -8,6 +8,7 @@ import sys
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # vocab_common.hpp kF32, kBF16, kF16
 _NOTHING = contextlib.nullcontext()
@@ -30,9 +31,10 @@ def _traced() -> bool:
 
 def no_grad_of(grad_name: str, *tensors) -> None:
     """These operators are not recorded by autograd; their gradients are
-    functions of their own.  A tensor that autograd follows is refused rather
-    than dropped out of its graph without a word, and so is a call that a
-    tracer records: it would see the output's allocation and no kernel."""
+    functions of their own.  A tensor that autograd follows, backwards or
+    forwards, is refused rather than dropped out of its graph without a word,
+    and so is a call that a tracer records: it would see the output's
+    allocation and no kernel."""
     if (_tracing() is not None or _modes() or _functions()) and _traced():
         raise ValueError("a tracer does not see what this operator computes: call it outside of torch.jit.trace, "
                          "make_fx and fake tensor modes")
@@ -40,6 +42,11 @@ def no_grad_of(grad_name: str, *tensors) -> None:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"autograd does not follow this operator: call it under torch.no_grad() or on a detached "
                              f"tensor, and {grad_name} for the gradient")
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("forward-mode differentiation does not follow this operator: call it on the primal "
+                                 "(torch.autograd.forward_ad.unpack_dual), without the tangent")
 
 
 def matrix(x: torch.Tensor, what: str) -> torch.Tensor:

@@ -1,10 +1,12 @@
 """What the operators on rows over a vocabulary, and the products beside them,
 refuse because a native call would go wrong on it without a word, and calls of
 theirs that take a path of their own."""
+import dataclasses
 import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils.flop_counter import FlopCounterMode
@@ -166,3 +168,42 @@ def test_compiled_callers_run_the_operators():
     f = torch.compile(step, backend="eager")
     for z in (o.z, o.z * 3.0):
         assert torch.equal(f(z, o.tok), step(z, o.tok))
+
+
+# ---- forward-mode differentiation -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", CALLS)
+def test_tangents_are_refused(dev, dtype, name):
+    o = Operands(dev, dtype)
+    with forward_ad.dual_level():
+        CALLS[name](o)                                        # tensors without a tangent
+        dual = o.change(lambda x: forward_ad.make_dual(x, torch.ones_like(x)))
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            CALLS[name](dual)
+        CALLS[name](dual.change(lambda x: forward_ad.unpack_dual(x).primal))
+    CALLS[name](o)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_each_tangent_is_refused(dev):
+    o = Operands(dev)
+    r, s = token_logprobs(o.z, o.tok), distill_loss(o.z, o.T)
+    with forward_ad.dual_level():
+        def d(x):
+            return forward_ad.make_dual(x, torch.ones_like(x))
+
+        calls = [lambda: embedding(o.W, o.tok, out=d(o.dY.clone())),
+                 lambda: embedding_grad(o.dY, o.tok, 7, out=d(o.W.clone()), accumulate=True),
+                 lambda: token_logprobs_grad(o.z, o.tok, r, d(o.g)),
+                 lambda: token_logprobs_grad(o.z, o.tok, r, None, d(o.g)),
+                 lambda: token_logprobs_grad(d(o.z), o.tok, r, o.g),
+                 lambda: token_logprobs_grad(o.z, o.tok, dataclasses.replace(r, stat=d(r.stat)), o.g),
+                 lambda: distill_loss_grad(o.z, o.T, weight=d(o.w)),
+                 lambda: distill_loss(o.z, o.T.with_values(d(o.T.val))),
+                 lambda: distill_grad(o.z, o.T, s, weight=d(o.w)),
+                 lambda: distill_grad(o.z, o.T, dataclasses.replace(s, saved=d(s.saved)))]
+        for call in calls:
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
