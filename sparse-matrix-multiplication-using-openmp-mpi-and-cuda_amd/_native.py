@@ -153,6 +153,8 @@ def ptr(t) -> int:
     if t is None:
         return None
     if hasattr(t, "data_ptr"):
+        if t.is_neg():
+            raise ValueError("a tensor whose negative bit is set has the negated values in memory: call resolve_neg()")
         return t.data_ptr() or null(t)
     return t.ctypes.data
 

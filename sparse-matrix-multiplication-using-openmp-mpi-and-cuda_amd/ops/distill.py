@@ -66,7 +66,7 @@ def _operands(logits: torch.Tensor, teacher: CSR):
     if val.dtype not in R.TYPES or val.shape != col.shape:
         raise ValueError(f"teacher.val must be float32, bfloat16 or float16 [{col.shape[0]}], got {val.dtype} "
                          f"{tuple(val.shape)}")
-    return z, n, V, ptr.contiguous(), col.contiguous(), val.contiguous()
+    return z, n, V, R.contiguous(ptr), R.contiguous(col), R.contiguous(val)
 
 
 def _run(logits, teacher, weight, temperature, out, gradient) -> Tuple[DistillLoss, Optional[torch.Tensor]]:
@@ -134,12 +134,13 @@ def distill_grad(logits: torch.Tensor, teacher: CSR, stats: DistillLoss, weight:
     if stats.rows != n or stats.entries != nnz:
         raise ValueError(f"stats are of {stats.rows} rows and {stats.entries} entries, the operands have {n} and {nnz}")
     inv_t = R.inverse_temperature(stats.temperature)
+    saved = R.contiguous(stats.saved)
     out = gradient_out(out, z)
     if n == 0:
         return out
     if not R.on_gpu(z):
         return _run(z, teacher, weight, stats.temperature, out, True)[1]
-    at, at_z, at_ptr = stats.saved.data_ptr() or null(stats.saved), z.data_ptr() or null(z), ptr.data_ptr() or null(ptr)
+    at, at_z, at_ptr = saved.data_ptr() or null(saved), z.data_ptr() or null(z), ptr.data_ptr() or null(ptr)
     at_col, at_val, at_out = col.data_ptr() or null(col), val.data_ptr() or null(val), out.data_ptr() or null(out)
     w = weight.data_ptr() or null(weight) if weight is not None else None
     with R.on(dev):

@@ -141,8 +141,7 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: Token
         raise ValueError(f"stats must be fp32 [4, {n}], got {stat.dtype} {tuple(stat.shape)}")
     if stat.shape[1] != n:
         raise ValueError(f"stats are of {stat.shape[1]} rows, the logits have {n}")
-    if not stat.is_contiguous():   # (some of a larger batch's rows)
-        stat = stat.contiguous()
+    stat = R.contiguous(stat)   # (some of a larger batch's rows)
     tok = R.token_ids(tokens)
     g, h = R.per_row(g_logprob, n, "g_logprob"), R.per_row(g_entropy, n, "g_entropy")
     inv_t = R.inverse_temperature(stats.temperature)

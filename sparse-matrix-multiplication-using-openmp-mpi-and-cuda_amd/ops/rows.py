@@ -49,6 +49,17 @@ def no_grad_of(grad_name: str, *tensors) -> None:
                                  "(torch.autograd.forward_ad.unpack_dual), without the tangent")
 
 
+def signed(x: torch.Tensor) -> torch.Tensor:
+    """x with its values in memory: a view may hold their negatives and a bit
+    that says so (the imaginary part of a conjugate does)."""
+    return x.resolve_neg() if x.is_neg() else x
+
+
+def contiguous(x: torch.Tensor) -> torch.Tensor:
+    x = signed(x)
+    return x if x.is_contiguous() else x.contiguous()
+
+
 def matrix(x: torch.Tensor, what: str) -> torch.Tensor:
     """x as [rows, columns] of one of the three types with adjacent columns
     (copied if they are not adjacent; any row stride)."""
@@ -56,6 +67,7 @@ def matrix(x: torch.Tensor, what: str) -> torch.Tensor:
         raise ValueError(f"{what} must have 2 dimensions, got {tuple(x.shape)}")
     if x.dtype not in TYPES:
         raise ValueError(f"{what} must be float32, bfloat16 or float16, got {x.dtype}")
+    x = signed(x)
     if x.stride(1) != 1 and x.shape[1] > 1:
         return x.contiguous()
     return x
@@ -79,7 +91,7 @@ def on_gpu(x: torch.Tensor) -> bool:
 def token_ids(tokens: torch.Tensor) -> torch.Tensor:
     if tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"tokens must be int32 or int64, got {tokens.dtype}")
-    return tokens if tokens.is_contiguous() else tokens.contiguous()
+    return contiguous(tokens)
 
 
 def per_row(x: Optional[torch.Tensor], n: int, what: str) -> Optional[torch.Tensor]:
@@ -92,7 +104,7 @@ def per_row(x: Optional[torch.Tensor], n: int, what: str) -> Optional[torch.Tens
         raise ValueError(f"{what} must be floating point, got {x.dtype}")
     if x.dtype != torch.float32:
         x = x.float()
-    return x.contiguous()
+    return contiguous(x)
 
 
 def output(out: torch.Tensor, shape, dtype: torch.dtype, device: torch.device, what: str = "out") -> None:
@@ -103,6 +115,8 @@ def output(out: torch.Tensor, shape, dtype: torch.dtype, device: torch.device, w
     if out.dtype != dtype:
         raise ValueError(f"{what} must be {dtype}, got {out.dtype}")
     same_device(device, **{what: out})
+    if out.is_neg():
+        raise ValueError(f"{what} must not have its negative bit set")
     if out.dim() == 2:
         n, d = out.shape
         if (d > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < d):

@@ -207,3 +207,74 @@ def test_each_tangent_is_refused(dev):
         for call in calls:
             with pytest.raises(ValueError, match="forward-mode"):
                 call()
+
+
+# ---- views that hold the negatives of their values ------------------------------------------------------------------
+
+def held_negated(x):
+    """x as the negative of what is in memory."""
+    y = torch._neg_view(-x)
+    assert y.is_neg() and torch.equal(y, x)
+    return y
+
+
+def results(r):
+    """All tensors of a result."""
+    if isinstance(r, torch.Tensor):
+        return [r]
+    if isinstance(r, tuple):
+        return [t for x in r for t in results(x)]
+    return [r.loss] if hasattr(r, "loss") else [r.logprob, r.entropy] + ([r.top.col, r.top.val] if r.top else [])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name", CALLS)
+def test_negated_views_are_their_values(dev, dtype, name):
+    o = Operands(dev, dtype)
+    for got, want in zip(results(CALLS[name](o.change(held_negated))), results(CALLS[name](o)), strict=True):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_negated_tokens_and_statistics_are_their_values(dev):
+    o = Operands(dev)
+    tok, r, s = held_negated(o.tok), token_logprobs(o.z, o.tok), distill_loss(o.z, o.T)
+    assert torch.equal(embedding(o.W, tok), o.W[o.tok])
+    assert torch.equal(embedding_grad(o.dY, tok, 7), embedding_grad(o.dY, o.tok, 7))
+    assert torch.equal(token_logprobs(o.z, tok).logprob, r.logprob)
+    want = token_logprobs_grad(o.z, o.tok, r, o.g, o.w)
+    assert torch.equal(token_logprobs_grad(o.z, tok, r, o.g, o.w), want)
+    stat = held_negated(r.stat[:4].clone())
+    assert torch.equal(token_logprobs_grad(o.z, o.tok, dataclasses.replace(r, stat=stat), o.g, o.w), want)
+    want = distill_grad(o.z, o.T, s, o.w)
+    saved = held_negated(s.saved[:5 * 3 + 5].clone())
+    assert torch.equal(distill_grad(o.z, o.T, dataclasses.replace(s, saved=saved), o.w), want)
+    T = CSR(3, 7, held_negated(o.T.rowptr), held_negated(o.T.col), o.T.val)
+    assert torch.equal(distill_loss_grad(o.z, T, o.w)[1], want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_negated_outputs_are_refused(dev):
+    o = Operands(dev)
+    r, s = token_logprobs(o.z, o.tok), distill_loss(o.z, o.T)
+    before = [x.clone() for x in (o.W, o.dY, o.z)]
+    for call in (lambda: embedding(o.W, o.tok, out=torch._neg_view(o.dY)),
+                 lambda: embedding_grad(o.dY, o.tok, 7, out=torch._neg_view(o.W)),
+                 lambda: embedding_grad(o.dY, o.tok, 7, out=torch._neg_view(o.W), accumulate=True),
+                 lambda: token_logprobs_grad(o.z, o.tok, r, o.g, out=torch._neg_view(o.z)),
+                 lambda: distill_loss_grad(o.z, o.T, out=torch._neg_view(o.z)),
+                 lambda: distill_grad(o.z, o.T, s, out=torch._neg_view(o.z))):
+        with pytest.raises(ValueError, match="negative bit"):
+            call()
+    assert all(torch.equal(a, b) for a, b in zip(before, (o.W, o.dY, o.z)))
+
+
+def test_the_imaginary_part_of_a_conjugate():
+    c = torch.randn(7, 9, dtype=torch.complex64, generator=torch.Generator().manual_seed(5))
+    W, tok = c.conj().imag, torch.tensor([1, 6, 0])
+    assert W.is_neg() and torch.equal(embedding(W, tok), -c.imag[tok])
+    X = torch.randn(7, 128, generator=torch.Generator().manual_seed(6))
+    A = Operands("cpu").T
+    with pytest.raises(ValueError, match="negative bit"):
+        spmm(A, torch._neg_view(X))
