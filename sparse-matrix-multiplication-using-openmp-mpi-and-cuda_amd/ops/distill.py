@@ -73,10 +73,11 @@ def _run(logits, teacher, weight, temperature, out, gradient) -> Tuple[DistillLo
     R.no_grad_of("distill_loss_grad", logits, weight, out, teacher.val)
     z, n, V, ptr, col, val = _operands(logits, teacher)
     dev, nnz, code = z.device, col.shape[0], R.TYPES[z.dtype]
-    R.same_device(dev, weight=weight)
-    weight = R.per_row(weight, n, "weight")
+    if weight is not None:
+        R.same_device(dev, weight=weight)
+        weight = R.per_row(weight, n, "weight")
     inv_t = R.inverse_temperature(temperature)
-    gpu = R.on_gpu(z)
+    gpu = z.is_cuda or not R.on_cpu(z)
     ws = _native.hip().spmm_vocab_ws(n, V, code, -1) if gpu else 0
     head = (5 * n + nnz + 3) // 4 * 4   # (the workspace starts at 16 bytes)
     saved = torch.empty(head + ws // 4, dtype=torch.float32, device=dev)
@@ -102,7 +103,7 @@ def _run(logits, teacher, weight, temperature, out, gradient) -> Tuple[DistillLo
         _native.check(_native.hip().spmm_distill(
             at_z, z.stride(0), n, V, code, at_ptr, at_col, at_val, R.TYPES[val.dtype], nnz, LOG2E * inv_t, inv_t, at,
             at + 4 * n, at + 20 * n, w, at_out, out.stride(0) if gradient else 0, at + 4 * head, ws,
-            _native.stream_ptr(dev)), "distill")
+            R.stream(dev)), "distill")
     return res, out
 
 
@@ -138,7 +139,7 @@ def distill_grad(logits: torch.Tensor, teacher: CSR, stats: DistillLoss, weight:
     out = gradient_out(out, z)
     if n == 0:
         return out
-    if not R.on_gpu(z):
+    if not z.is_cuda and R.on_cpu(z):
         return _run(z, teacher, weight, stats.temperature, out, True)[1]
     at, at_z, at_ptr = saved.data_ptr() or null(saved), z.data_ptr() or null(z), ptr.data_ptr() or null(ptr)
     at_col, at_val, at_out = col.data_ptr() or null(col), val.data_ptr() or null(val), out.data_ptr() or null(out)
@@ -146,5 +147,5 @@ def distill_grad(logits: torch.Tensor, teacher: CSR, stats: DistillLoss, weight:
     with R.on(dev):
         _native.check(_native.hip().spmm_distill_grad(
             at_z, z.stride(0), n, V, R.TYPES[z.dtype], at_ptr, at_col, at_val, R.TYPES[val.dtype], nnz, LOG2E * inv_t,
-            inv_t, at + 4 * n, at + 20 * n, w, at_out, out.stride(0), _native.stream_ptr(dev)), "distill_grad")
+            inv_t, at + 4 * n, at + 20 * n, w, at_out, out.stride(0), R.stream(dev)), "distill_grad")
     return out

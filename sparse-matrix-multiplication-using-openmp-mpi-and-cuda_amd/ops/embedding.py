@@ -53,7 +53,7 @@ def embedding(W: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
     W = R.matrix(W, "W")
     dev = W.device
     R.same_device(dev, tokens=tokens)
-    gpu = R.on_gpu(W)
+    gpu = W.is_cuda or not R.on_cpu(W)
     tok = R.token_ids(tokens)
     scale = _scale(scale)
     V, D = W.shape
@@ -78,7 +78,7 @@ def embedding(W: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
     with R.on(dev):
         _native.check(_native.hip().spmm_embedding(at_w, W.stride(0), V, D, R.TYPES[W.dtype], at_tok,
                                                    tok.dtype == torch.int64, n, scale, at_y, y.stride(0),
-                                                   _native.stream_ptr(dev)), "embedding")
+                                                   R.stream(dev)), "embedding")
     return out
 
 
@@ -101,7 +101,7 @@ def embedding_grad(dY: torch.Tensor, tokens: torch.Tensor, V: int, scale: float 
     D, n = dY.shape[-1], tokens.numel()
     dev = dY.device
     R.same_device(dev, tokens=tokens)
-    gpu = R.on_gpu(dY)
+    gpu = dY.is_cuda or not R.on_cpu(dY)
     dy = R.matrix(dY if dY.dim() == 2 else dY.reshape(n, D), "dY")
     tok = R.token_ids(tokens)
     scale = _scale(scale)
@@ -134,6 +134,6 @@ def embedding_grad(dY: torch.Tensor, tokens: torch.Tensor, V: int, scale: float 
         ws = torch.empty(bytes_, dtype=torch.uint8, device=dev) if bytes_ else None
         _native.check(lib.spmm_embedding_grad(at_dy, dy.stride(0), R.TYPES[dy.dtype], at_tok, tok.dtype == torch.int64,
                                               n, V, D, scale, at_out, out.stride(0), R.TYPES[dtype], accumulate,
-                                              ws.data_ptr() if bytes_ else None, bytes_, _native.stream_ptr(dev)),
+                                              ws.data_ptr() if bytes_ else None, bytes_, R.stream(dev)),
                       "embedding_grad")
     return out

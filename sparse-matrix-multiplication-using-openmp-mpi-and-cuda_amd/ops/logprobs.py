@@ -85,7 +85,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     k = int(k)
     if not 0 <= k <= min(MAX_TOP, V):
         raise ValueError(f"k must be between 0 and {min(MAX_TOP, V)}, got {k}")
-    on_gpu = R.on_gpu(z)
+    on_gpu = z.is_cuda or not R.on_cpu(z)
     gpu = on_gpu and n > 0
     bytes_ = _native.hip().spmm_vocab_ws(n, V, R.TYPES[z.dtype], k) if gpu else 0
     kept = bytes_ <= KEPT   # (a row's workspace is whole floats, and starts at 16 bytes)
@@ -115,7 +115,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
         _native.check(_native.hip().spmm_token_logprobs(
             at_z, z.stride(0), n, V, R.TYPES[z.dtype], at_tok, tok.dtype == torch.int64, k,
             LOG2E * inv_t, inv_t, at_stat, *at, at_stat + 16 * n if kept else ws.data_ptr(), bytes_,
-            _native.stream_ptr(dev)), "token_logprobs")
+            R.stream(dev)), "token_logprobs")
     return res
 
 
@@ -130,7 +130,7 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: Token
     logits are not read."""
     R.no_grad_of("token_logprobs_grad", logits, stats.stat, g_logprob, g_entropy, out)
     z = logits_rows(logits)
-    gpu = R.on_gpu(z)
+    gpu = z.is_cuda or not R.on_cpu(z)
     n, V = z.shape
     dev = z.device
     R.same_device(dev, tokens=tokens, g_logprob=g_logprob, g_entropy=g_entropy, stats=stats.stat)
@@ -163,5 +163,5 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: torch.Tensor, stats: Token
     with R.on(dev):
         _native.check(_native.hip().spmm_token_logprobs_grad(
             at_z, z.stride(0), n, V, R.TYPES[z.dtype], at_tok, tok.dtype == torch.int64, LOG2E * inv_t, inv_t, at_stat,
-            at_g, at_h, at_out, out.stride(0), _native.stream_ptr(dev)), "token_logprobs_grad")
+            at_g, at_h, at_out, out.stride(0), R.stream(dev)), "token_logprobs_grad")
     return out

@@ -49,14 +49,12 @@ def no_grad_of(grad_name: str, *tensors) -> None:
                                  "(torch.autograd.forward_ad.unpack_dual), without the tangent")
 
 
-def signed(x: torch.Tensor) -> torch.Tensor:
-    """x with its values in memory: a view may hold their negatives and a bit
-    that says so (the imaginary part of a conjugate does)."""
-    return x.resolve_neg() if x.is_neg() else x
-
+# (A view may hold the negatives of its values and a bit that says so, as the imaginary part of a
+# conjugate does: resolve_neg() puts the values in memory.)
 
 def contiguous(x: torch.Tensor) -> torch.Tensor:
-    x = signed(x)
+    if x.is_neg():
+        x = x.resolve_neg()
     return x if x.is_contiguous() else x.contiguous()
 
 
@@ -67,8 +65,9 @@ def matrix(x: torch.Tensor, what: str) -> torch.Tensor:
         raise ValueError(f"{what} must have 2 dimensions, got {tuple(x.shape)}")
     if x.dtype not in TYPES:
         raise ValueError(f"{what} must be float32, bfloat16 or float16, got {x.dtype}")
-    x = signed(x)
-    if x.stride(1) != 1 and x.shape[1] > 1:
+    if x.is_neg():
+        x = x.resolve_neg()
+    if x.stride()[1] != 1 and x.shape[1] > 1:
         return x.contiguous()
     return x
 
@@ -79,19 +78,19 @@ def same_device(device: torch.device, **others) -> None:
             raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
 
 
-def on_gpu(x: torch.Tensor) -> bool:
-    """Whether x's operators run on the GPU, as opposed to the CPU: there are no others."""
-    if x.is_cuda:
-        return True
+def on_cpu(x: torch.Tensor) -> bool:
+    """True; operands that are neither on a GPU nor on the CPU are refused."""
     if not x.is_cpu:
         raise ValueError(f"operands must be on the CPU or a GPU, got {x.device}")
-    return False
+    return True
 
 
 def token_ids(tokens: torch.Tensor) -> torch.Tensor:
     if tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"tokens must be int32 or int64, got {tokens.dtype}")
-    return contiguous(tokens)
+    if tokens.is_neg():
+        tokens = tokens.resolve_neg()
+    return tokens if tokens.is_contiguous() else tokens.contiguous()
 
 
 def per_row(x: Optional[torch.Tensor], n: int, what: str) -> Optional[torch.Tensor]:
@@ -160,6 +159,8 @@ def inverse_temperature(temperature: float) -> float:
 
 def on(device: torch.device):
     """Launches go to the current device: make it the operands'."""
-    if device.index == torch._C._cuda_getDevice():
-        return _NOTHING
-    return torch.cuda.device(device)
+    return _NOTHING if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
