@@ -135,7 +135,10 @@ def distill_grad(logits: torch.Tensor, teacher: CSR, stats: DistillLoss, weight:
     if stats.rows != n or stats.entries != nnz:
         raise ValueError(f"stats are of {stats.rows} rows and {stats.entries} entries, the operands have {n} and {nnz}")
     inv_t = R.inverse_temperature(stats.temperature)
-    saved = R.contiguous(stats.saved)
+    saved = stats.saved
+    if saved.dtype != torch.float32 or saved.dim() != 1 or saved.shape[0] < 5 * n + nnz:
+        raise ValueError(f"stats.saved must be fp32 [{5 * n + nnz}] or longer, got {saved.dtype} {tuple(saved.shape)}")
+    saved = R.contiguous(saved)
     out = gradient_out(out, z)
     if n == 0:
         return out

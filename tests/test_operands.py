@@ -278,3 +278,19 @@ def test_the_imaginary_part_of_a_conjugate():
     A = Operands("cpu").T
     with pytest.raises(ValueError, match="negative bit"):
         spmm(A, torch._neg_view(X))
+
+
+# ---- statistics of the distillation ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_statistics_that_are_not_the_losses_are_refused(dev):
+    """The kernel reads 5 numbers a row and one an entry from them."""
+    o = Operands(dev)
+    s = distill_loss(o.z, o.T)
+    want = distill_grad(o.z, o.T, s, o.w)
+    for saved in (s.saved[:5 * 3 + 4], s.loss, s.saved.bfloat16(), s.saved.double(), s.saved[:16].view(4, 4)):
+        with pytest.raises(ValueError, match="stats.saved must be"):
+            distill_grad(o.z, o.T, dataclasses.replace(s, saved=saved), o.w)
+    apart = torch.stack([s.saved, s.saved], dim=1)[:, 0]
+    for saved in (s.saved[:5 * 3 + 5].clone(), apart):
+        assert torch.equal(distill_grad(o.z, o.T, dataclasses.replace(s, saved=saved), o.w), want)
