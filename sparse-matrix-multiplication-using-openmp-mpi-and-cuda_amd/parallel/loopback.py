@@ -259,17 +259,15 @@ class PanelComm(Comm):
     and none of this GPU's CUs copy them.  ``tools/rank_emulate.py`` models a
     rank of an N-GPU node with it; tests drive the W-rank branches with it."""
 
-    def __init__(self, rank: int, world: int, dev: torch.device, panels, gbps: float = 0.0, link_priority: int = 0,
+    def __init__(self, rank: int, world: int, dev: torch.device, panels, gbps: float = 0.0, *,
                  prefill: bool = False):
         super().__init__(rank, world, rank, dev, "panels")
         if len(panels) != world:
             raise ValueError("PanelComm: one B panel per rank")
         self.panels, self.gbps, self.prefill = panels, gbps, prefill
         self._filled = set()
-        # (``link_priority`` -1: high-priority streams, whose work the dispatcher puts
-        # ahead of the compute stream's large grids; tools/rank_emulate.py --link-priority)
-        self.link = torch.cuda.Stream(dev, priority=link_priority) if dev.type == "cuda" else None
-        self.wire = torch.cuda.Stream(dev, priority=link_priority) if dev.type == "cuda" else None
+        self.link = torch.cuda.Stream(dev) if dev.type == "cuda" else None
+        self.wire = torch.cuda.Stream(dev) if dev.type == "cuda" else None
         self._n = 0
         self._payloads = None
 

@@ -24,8 +24,7 @@ SPMM_STAMPS_PREBUILT=1 timeout -k 10 300 python -u tools/bm_wg_times.py --world 
 SPMM_STAMPS_PREBUILT=1 timeout -k 10 300 python -u tools/bm_wg_times.py --world 1 > $O/wg1.json 2> $O/wg1.err || { tail -20 $O/wg1.err; exit 1; }
 cat $O/wg8.json $O/wg1.json
 timeout -k 10 400 python -u tools/rank_emulate.py --world 8 --rank 0 --graph --gather-gbps 0,300 > $O/emu8.json 2> $O/emu8.err || { tail -20 $O/emu8.err; exit 1; }
-timeout -k 10 400 python -u tools/rank_emulate.py --world 8 --rank 0 --no-local --gather-gbps 300 --link-priority -1 > $O/emu8_hi.json 2> $O/emu8_hi.err || { tail -20 $O/emu8_hi.err; exit 1; }
-cat $O/emu8.json $O/emu8_hi.json
+cat $O/emu8.json
 timeout -k 10 600 python -u -m pytest -x -v --timeout 300 --timeout-method thread -p no:cacheprovider -m gpu \
   tests/test_dist_device.py tests/test_spgemm.py -k "panel_comm or rowblock_graph or rccl_one_rank" > $O/pytest_b.log 2>&1 || { tail -40 $O/pytest_b.log; exit 1; }
 echo "tests b: $(tail -1 $O/pytest_b.log)"

@@ -1,5 +1,5 @@
 #!/bin/bash
-# R-MAT overlap with a high-priority side stream: tests, bench + allocator counters, kernel trace windows
+# R-MAT overlap with the side stream: tests, bench + allocator counters, kernel trace windows
 set -o pipefail
 R=${GRAFT_REPO_ROOT:-/root/repo}
 O=$R/gpurun_out/r6g42; mkdir -p $O

@@ -63,8 +63,6 @@ def main() -> None:
     ap.add_argument("--graph", action="store_true", help="time the local product as a SpgemmGraph replay")
     ap.add_argument("--gather-gbps", default="", help="comma list: emulate the whole step at these link rates")
     ap.add_argument("--no-local", action="store_true", help="skip the local-product timings")
-    ap.add_argument("--link-priority", type=int, default=0,
-                    help="stream priority of the emulated link (-1: high, dispatched ahead of the compute grids)")
     a = ap.parse_args()
     dev = torch.device("cuda", 0)
     _native.hip()
@@ -91,7 +89,7 @@ def main() -> None:
         keep = []   # (graphs stay alive until the end: see tests/test_dist_device.py _graph_case_panels)
         for g in [float(x) for x in a.gather_gbps.split(",")]:
             for prefill, d in ((False, steps), (True, link)):
-                comm = PanelComm(a.rank, a.world, dev, panels, g, link_priority=a.link_priority, prefill=prefill)
+                comm = PanelComm(a.rank, a.world, dev, panels, g, prefill=prefill)
                 rg = MS.RowblockGraph(A, panels[a.rank], comm)
                 d[str(g)] = round(timed(rg.run, a.steps), 3)
                 C = rg.result()
