@@ -961,3 +961,57 @@ def test_refusals_logits(dev):
     if dev == "cuda":
         refused(lambda: distill_loss(z, T.to("cpu")), "is on")
         refused(lambda: token_logprobs(z, tok.cpu()), "is on")
+
+
+# ---- distillation: rows that fill a CU's registers, teacher rows against a large vocabulary --------------------------
+
+def teacher_with_equal_columns(n, V, least, most, seed):
+    """Rows of `least` to `most` entries in any order, with columns twice in a
+    row's first 64 entries and further apart, one of them three times, and
+    absent entries."""
+    g = gen(seed)
+    rows = []
+    for i in range(n):
+        L = least + int(torch.randint(0, most - least + 1, (1,), generator=g))
+        c = torch.randperm(V, generator=g)[:L]
+        c[L - 1] = c[3]
+        c[7] = c[3]
+        c[L // 2] = c[L - 2]
+        c[20] = c[21]
+        c[30] = c[L - 4] = -1
+        c[0], c[L - 3] = 0, V - 1                            # beside the row's vectors
+        rows.append([(int(x), float(v)) for x, v in zip(c, torch.randn(L, generator=g) * 2)])
+    return teacher_of(rows, V)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,V", [(260, 40001), (256, 65532), (257, 33024)])
+def test_distill_rows_that_fill_a_cu(dtype, n, V):
+    """16-bit rows of 17 to 32 pages, many of them: a workgroup of 1024 threads holds one."""
+    z, _ = logits(n, V, dtype, seed=50)
+    z[5, 17:9000] = -math.inf
+    w = torch.rand(n, generator=gen(51)) + 0.1
+    w[3] = 0.0
+    check_distill(z, random_teacher(n, V, 90, seed=V), 1.5, w, "cuda")
+    check_distill(z, teacher_with_equal_columns(n, V, 66, 200, seed=52), 1.0, w, "cuda", inplace=True)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_equal_columns_in_a_large_vocabulary(dev, dtype):
+    """65 to 128 entries against 300001 columns: equal ones are found by a search among all entries."""
+    z, _ = logits(3, 300001, dtype, seed=53)
+    w = torch.tensor([0.5, 1.25, 2.0])
+    for seed in (54, 55):
+        T = teacher_with_equal_columns(3, 300001, 65, 128, seed=seed)
+        check_distill(z, T, 1.3, w, dev)
+        check_distill(z, T, 1.0, None, dev, inplace=True)
+
+
+@pytest.mark.gpu
+def test_distill_equal_columns_of_many_rows_in_a_large_vocabulary():
+    """The same where a launch of its own ends the rows."""
+    z, _ = logits(40, 300001, torch.float32, seed=56)
+    w = torch.rand(40, generator=gen(57)) + 0.1
+    check_distill(z, teacher_with_equal_columns(40, 300001, 65, 128, seed=58), 1.3, w, "cuda", inplace=True)
