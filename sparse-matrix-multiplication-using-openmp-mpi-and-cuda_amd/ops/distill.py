@@ -58,7 +58,9 @@ def _operands(logits: torch.Tensor, teacher: CSR):
     ptr, col, val = teacher.rowptr, teacher.col, teacher.val
     if teacher.m != n or teacher.n != V:
         raise ValueError(f"the teacher is {teacher.m} x {teacher.n}, the logits {n} x {V}")
-    R.same_device(z.device, teacher=ptr, teacher_col=col, teacher_val=val)
+    dev = z.device
+    if ptr.device != dev or col.device != dev or val.device != dev:
+        R.same_device(dev, teacher=ptr, teacher_col=col, teacher_val=val)
     if ptr.dtype != torch.int64 or ptr.dim() != 1 or ptr.shape[0] != n + 1:
         raise ValueError(f"teacher.rowptr must be int64 [{n + 1}], got {ptr.dtype} {tuple(ptr.shape)}")
     if col.dtype != torch.int32 or col.dim() != 1:

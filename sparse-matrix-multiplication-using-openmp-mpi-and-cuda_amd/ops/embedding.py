@@ -18,7 +18,6 @@ both directions can be captured into a HIP graph.
 from __future__ import annotations
 
 import ctypes as C
-import math
 from typing import Optional
 
 import torch
@@ -37,7 +36,7 @@ _native.register_hip("spmm_embedding_grad", c_vp, C.c_int64, C.c_int, c_vp, C.c_
 
 def _scale(scale: float) -> float:
     s = float(scale)
-    if not math.isfinite(s) or abs(s) > 3e38:
+    if not -3e38 <= s <= 3e38:
         raise ValueError(f"scale must be finite, got {scale}")
     return s
 
@@ -52,7 +51,8 @@ def embedding(W: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
     R.no_grad_of("embedding_grad", W)
     W = R.matrix(W, "W")
     dev = W.device
-    R.same_device(dev, tokens=tokens)
+    if tokens.device != dev:
+        R.same_device(dev, tokens=tokens)
     gpu = W.is_cuda or not R.on_cpu(W)
     tok = R.token_ids(tokens)
     scale = _scale(scale)
@@ -100,7 +100,8 @@ def embedding_grad(dY: torch.Tensor, tokens: torch.Tensor, V: int, scale: float 
         raise ValueError(f"dY must be {tuple(tokens.shape)} + (D,), got {tuple(dY.shape)}")
     D, n = dY.shape[-1], tokens.numel()
     dev = dY.device
-    R.same_device(dev, tokens=tokens)
+    if tokens.device != dev:
+        R.same_device(dev, tokens=tokens)
     gpu = dY.is_cuda or not R.on_cpu(dY)
     dy = R.matrix(dY if dY.dim() == 2 else dY.reshape(n, D), "dY")
     tok = R.token_ids(tokens)

@@ -77,7 +77,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     z = logits_rows(logits)
     n, V = z.shape
     dev = z.device
-    R.same_device(dev, tokens=tokens)
+    if tokens.device != dev:
+        R.same_device(dev, tokens=tokens)
     if tokens.dim() != 1 or tokens.shape[0] != n:
         raise ValueError(f"tokens must be [{n}], got {tuple(tokens.shape)}")
     tok = R.token_ids(tokens)

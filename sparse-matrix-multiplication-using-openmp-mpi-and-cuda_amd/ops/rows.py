@@ -3,7 +3,6 @@
 from __future__ import annotations
 
 import contextlib
-import math
 import sys
 from typing import Optional
 
@@ -152,7 +151,7 @@ def apart(out: torch.Tensor, x: torch.Tensor, what: str, in_place: bool) -> None
 
 def inverse_temperature(temperature: float) -> float:
     t = float(temperature)
-    if not (math.isfinite(t) and 1e-30 < t < 1e30):
+    if not 1e-30 < t < 1e30:
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
     return 1.0 / t
 
