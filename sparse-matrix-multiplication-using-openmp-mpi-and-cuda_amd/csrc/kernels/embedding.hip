@@ -370,11 +370,15 @@ struct GradArgs {
   int brief;                // embed_grad_brief, without sorted entries
 };
 
-// Sorted entries a wave sums.  Few waves have little to hide their loads behind:
-// 3000 tokens of 500 columns take 26 us with 8 entries a wave, 31 with 16 and 43
-// with 32; 20548 of 857 53, 53 and 60; 12000 of 4096 87, 81 and 79.  One token
-// only, whose partial rows are joined by one workgroup: 41, 33 and 32 us for 4000
-// of 128 columns, 194, 114 and 77 for 32000 of 256.
+// Sorted entries a wave sums.  A wave hides its loads behind those of other
+// waves, so it gets few entries where the chip's 1024 SIMDs would have few waves
+// otherwise: up to 6144 tokens times slices waves of 8 are at most 768, up to
+// 65536 waves of 16 at most 4096, and above that waves of 32 at least 2048.  The
+// whole gradient of mixed tokens with 8, 16 and 32 entries a wave: 3000 of 500
+// columns 25, 31 and 41 us; 32000 of 256 47, 45 and 48; 20548 of 857 54, 55 and
+// 59; 12000 of 4096 90, 82 and 79; 65536 of 1024 110, 98 and 90.  A token that
+// fills much of the batch asks for more, as one workgroup a slice joins its
+// partial rows: half of the 32000 117, 80 and 66 us, all of them 199, 118 and 80.
 inline int64_t tile_of(int64_t entries) {   // tokens times slices
   return entries <= 6144 ? 8 : entries <= 65536 ? 16 : 32;
 }
@@ -663,8 +667,12 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_grad_join(GradArgs a) {
 // token among all of them and, if it is the first such place, sums the rows in
 // order: no sort, one launch, and one before it that zeroes the table.  1000
 // tokens over 8192 x 1024 bf16: 10.3 us (sorted: 16.1), added to an fp32 table
-// 6.3 (15.2); 777 of mixed frequency over 32003 x 1000 16.1 (22.3).  One token
-// only, which no batch is: 777 times 49 (24.5).
+// 6.3 (15.2); 777 of mixed frequency over 32003 x 1000 15.7 (22.3).  A token's
+// rows are summed by one workgroup a slice however many they are, and where one
+// token (a pad id of its own, a placeholder) is much of the batch that takes
+// longer than the sort: a quarter, half, three quarters and all of the 777 21,
+// 31, 40 and 48 us (23, 24, 24 and 24), of the 1000 12, 17, 24 and 29 (18, 19, 21
+// and 20).
 constexpr int kBriefTokens = 1024;
 constexpr int64_t kBriefGroups = 4096;   // two rounds of the chip
 constexpr int kBriefWaves = 8, kBriefFlight = 8;   // 4 waves: a run of 777 112 us; 16 rows in flight: 1000 x 1024 20

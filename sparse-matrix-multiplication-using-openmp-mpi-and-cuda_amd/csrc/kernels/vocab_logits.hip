@@ -1045,9 +1045,10 @@ __global__ __launch_bounds__(kThreads) void distill_finish(DistillArgs a) {
 }
 
 // Rows that one workgroup holds in registers: loss, statistics and, with an
-// output, the gradient in one launch that reads the logits once (4096 x 32768
-// bf16: 116 us instead of 151, 256 x 16000 12 instead of 16).  A row's steps wait
-// for each other, which costs most where a workgroup fills the CU.
+// output, the gradient in one launch that reads the logits once (GPU time of loss
+// and gradient, bf16: 4096 x 32768 113 us instead of 147, 256 x 16000 10.6 instead
+// of 14.3, 8000 x 16000 112 instead of 183).  A row's steps wait for each other,
+// which costs most where a workgroup fills the CU.
 template <typename T, int VPT, int THREADS>
 __global__ __launch_bounds__(THREADS) void distill_rows(DistillArgs a) {
   constexpr int N = Elem<T>::kN;
@@ -1142,7 +1143,9 @@ void launch_grad(const DistillArgs& a, const Plan& q, hipStream_t s) {
 // distill_rows, or false where the other launches are better: the loss alone has
 // no second read to save (1024 rows of 8000 bf16 7.4 us instead of 8.6, 2048 12.9
 // instead of 11.9), and a workgroup of 16 waves leaves the chip empty in a short
-// call (128 x 65536 bf16 16.4 us instead of 14.8, 256 17.8 instead of 22.6).
+// call (128 x 65536 bf16 16.4 us instead of 14.8, 256 17.2 instead of 22.3).  So
+// does one of 8 waves with few rows: 48 x 32768 fp16 take 11.5 us on the GPU and
+// 9.3 in two launches, but a call 14.6 instead of 17.3, as the host bounds it.
 template <typename T>
 bool launch_rows(const DistillArgs& a, int type, hipStream_t s) {
   const int64_t pages = pages_of(a.V, type);
